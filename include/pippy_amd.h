@@ -341,6 +341,78 @@ int pp_moe_gate_bwd(const void* dout, int64_t ld_dout, const void* y, int64_t ld
                     const int32_t* topk_idx, const float* gate, int topk, int E, void* dlogits,
                     int64_t ld_dl, int64_t T, int64_t C, pp_stream stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Routing to experts in general form (the router of a mixture-of-experts layer inside the stage module; forward
+ * through pippy/_PipelineStage.py:420-428, backward through pippy/_backward.py:67-69).  Per token, with E logits:
+ *   score s_e: softmax over the experts, or 1 / (1 + exp(-logit));   choice c_e = s_e + bias_e (bias null: 0)
+ *   n_group > 1: the experts are n_group runs of E / n_group neighbours; a group's score is its largest choice
+ *   (PP_MOE_GROUP_MAX) or the sum of its two largest (PP_MOE_GROUP_TOP2), and only the topk_group best groups
+ *   stay open (ties: the lower group)
+ *   topk_idx[t, :]: the topk largest choices of open groups, descending, ties to the lower expert; choices are
+ *   compared in 64 bits (without a bias the logits themselves are compared)
+ *   gate[t, k] = scale * s[idx_k] / (renorm ? sum_j s[idx_j] : 1)         (a sum of 0 gives gates of 0)
+ * A logit of -infinity takes its expert out: it is not selected and counts in no sum; a token with fewer than
+ * topk experts left has topk_idx -1 and gate 0 in its last slots, which the permutations drop (position -1).  A
+ * NaN logit makes the token's softmax weights NaN and ranks behind every number.
+ * Backward: the gradient of the logits from dgate (fp32 [T, topk]), or, with dgate null, from
+ * dgate[t, k] = <dout[t, :], y[pos[t, k], :]> formed on the way (dout bf16 [T, C], y the bf16 expert rows, pos as
+ * pp_moe_permute gives it; a negative position or index counts as no contribution).  The bias gets no gradient.
+ * dlogits has the type of logits; its columns E .. cols_dl - 1 are written as zeros.
+ * 2 <= E <= 512, topk <= 16, n_group <= 64.  Rows of logits and dlogits need no alignment.
+ * ---------------------------------------------------------------------------------------- */
+enum pp_moe_scoring { PP_MOE_SOFTMAX = 0, PP_MOE_SIGMOID = 1 };
+enum pp_moe_group_score { PP_MOE_GROUP_MAX = 0, PP_MOE_GROUP_TOP2 = 1 };
+typedef struct pp_moe_route_desc {
+    const void* logits;   /* [T, E], row stride ld elements, dtype PP_BF16 or PP_F32 */
+    int64_t ld, T;
+    const float* bias;    /* forward: fp32 [E] or null */
+    int32_t* topk_idx;    /* [T, topk]: written by the forward, read by the backward */
+    float* gate;          /* forward: fp32 [T, topk] */
+    int32_t dtype, E, topk;
+    int32_t scoring;      /* enum pp_moe_scoring */
+    int32_t n_group;      /* forward: 0 or 1: no groups */
+    int32_t topk_group;
+    int32_t group_score;  /* enum pp_moe_group_score */
+    int32_t renorm;
+    float scale;
+    int32_t cols_dl;      /* backward: columns of dlogits to write, E <= cols_dl <= 512 */
+    const float* dgate;   /* backward: fp32 [T, topk], or null: from dout, y and pos */
+    const void* dout; const void* y; const int32_t* pos;
+    int64_t ld_dout, ld_y, C;
+    void* dlogits;        /* backward: [T, cols_dl], row stride ld_dl */
+    int64_t ld_dl;
+} pp_moe_route_desc;
+int pp_moe_route(const pp_moe_route_desc* desc, pp_stream stream);
+int pp_moe_route_bwd(const pp_moe_route_desc* desc, pp_stream stream);
+
+/* pp_moe_permute for up to 1024 experts and many slots: the same outputs bit for bit, on as many work-groups as
+ * the slots fill.  workspace: pp_moe_permute_workspace_ints(n_slots, E) int32, not shared by calls that may
+ * overlap; that function returns -1 for sizes out of range.  (index_add_ / sort of the torch form of the block,
+ * pippy/_PipelineStage.py:420-428.) */
+int64_t pp_moe_permute_workspace_ints(int64_t n_slots, int E);
+int pp_moe_permute_ws(const int32_t* expert_of_slot, int64_t n_slots, int E, int32_t* seg_start, int32_t* row_src,
+                      int32_t* pos, int32_t* workspace, int64_t workspace_ints, pp_stream stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Dropout with an optional residual (F.dropout and the addition that follows it inside the stage module; backward
+ * through pippy/_backward.py:67-69).  The mask is a function of {seed, offset, site, element index} and is
+ * formed again in the backward instead of being stored:
+ *   y = (resid ? resid : 0) + m x / (1 - p'),    dx = m dy / (1 - p')       (the residual's gradient is dy itself)
+ * border = round(65536 p), p' = border / 65536; element i (row-major over [rows, C]) stays (m = 1) when its 16-bit
+ * draw is >= border; the draws of elements 8 g .. 8 g + 7 are the low and high halves of the four words of
+ * Philox4x32-10 on the counter {g, offset low, offset high, site} under the key {seed low, seed high}.  p = 1 drops
+ * everything.  A dropped element contributes zero whatever it holds.
+ * rng: DEVICE memory, {seed, offset}, read when the kernel runs; calls that may mask alike by accident (layers, the
+ * two dropouts of a layer) use different sites, steps and microbatches different offsets (pp_rng_advance adds to
+ * the offset on the stream).  dtype PP_BF16 or PP_F32; 16-byte aligned pointers; with one row C is any length, with
+ * several rows C and the leading dimensions are multiples of 8; y may be x or resid.
+ * ---------------------------------------------------------------------------------------- */
+int pp_dropout_add(const void* x, int64_t ld_x, const void* resid, int64_t ld_resid, void* y, int64_t ld_y,
+                   int64_t rows, int64_t C, int dtype, float p, const uint64_t* rng, uint32_t site, pp_stream stream);
+int pp_dropout_bwd(const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx, int64_t rows, int64_t C, int dtype, float p,
+                   const uint64_t* rng, uint32_t site, pp_stream stream);
+int pp_rng_advance(uint64_t* rng, uint64_t step, pp_stream stream);
+
 /* Column reductions of one weight-gradient pass in two launches.  Per descriptor:
  *   out_sum[c] = sum_r dy[r, c]                                   (bias gradient / dbeta), and, if
  *   out_dot is non-null, out_dot[c] = sum_r dy[r, c] * (x[r, c] - mean[r]) * rstd[r]   (dgamma).
@@ -439,6 +511,43 @@ typedef struct pp_attn_desc {
 #define PP_ATTN_EXACT_DQ 1
 int pp_attn_fwd(const pp_attn_desc* desc, pp_stream stream);
 int pp_attn_bwd(const pp_attn_desc* desc, pp_stream stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention over packed sequences of different lengths (what a stage module computes per sequence with
+ * F.scaled_dot_product_attention, pippy/_PipelineStage.py:420-428, backward pippy/_backward.py:67-69, without the
+ * padding that equal lengths would need).  The T rows hold n_seq sequences one after the other, sequence b in rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (ascending int32 in device memory; empty sequences are fine; bounds out of
+ * order or outside [0, T] make an empty sequence).  Any length from 1; causal: query i of a sequence sees its keys
+ * 0 .. i, else all its keys.  Rows that belong to no sequence are neither read nor written.
+ * q: bf16, element (t, h, d) at q + t * stride_q + h * D + d, likewise o, d_o, dq (H heads) and k, v, dk, dv (Hkv
+ * heads; query head h reads key / value head h / (H / Hkv), whose gradients are sums over the group in ascending
+ * head order).  Row strides are multiples of 8 elements, at most 2^23, pointers 16-byte aligned: q, k, v may be
+ * sections of one projection's rows.  lse, delta: fp32 [H, T] (log-sum-exp of the scaled scores, saved for the
+ * backward; the backward's row sums of P dP).  D 64 or 128.  scale > 0.  Softmax statistics and all sums are fp32;
+ * P and dS are rounded to bf16 as operands of their products.  No atomics: the same bits on every run.
+ * A non-finite value row reaches, besides the queries that see it, earlier queries of its block of rows (0 * NaN
+ * inside a matrix product), never another sequence.
+ *
+ * The plan says which blocks of rows there are, longest first.  pp_attn_packed_plan builds it on the device from
+ * cu_seqlens (one small launch, no host synchronisation); every layer and both directions of a batch share it.
+ * plan: int32 [pp_attn_packed_plan_ints(n_seq, T)], 16-byte aligned; n_seq and T of a call must be the plan's.
+ * ---------------------------------------------------------------------------------------- */
+typedef struct pp_attn_packed_desc {
+    const void* q; const void* k; const void* v;
+    void* o; float* lse;
+    const void* d_o;               /* backward only */
+    void* dq; void* dk; void* dv;  /* backward only */
+    float* delta;                  /* backward workspace */
+    const int32_t* plan;
+    int64_t n_seq, T, H, Hkv, D;
+    int64_t stride_q, stride_k, stride_v, stride_o, stride_do, stride_dq, stride_dk, stride_dv; /* elements */
+    float scale;
+    int32_t causal;
+} pp_attn_packed_desc;
+int64_t pp_attn_packed_plan_ints(int64_t n_seq, int64_t T); /* -1: out of range */
+int pp_attn_packed_plan(const int32_t* cu_seqlens, int64_t n_seq, int64_t T, int32_t* plan, pp_stream stream);
+int pp_attn_packed_fwd(const pp_attn_packed_desc* desc, pp_stream stream);
+int pp_attn_packed_bwd(const pp_attn_packed_desc* desc, pp_stream stream);
 
 /* ------------------------------------------------------------------------------------------
  * Token + position embedding (F.embedding inside the first stage).

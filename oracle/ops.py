@@ -168,3 +168,83 @@ def moe_top2(x, w_router, w1, w2, w3, idx=None):
         ye = F.linear(swiglu(F.linear(xe, w1[e]), F.linear(xe, w3[e])), w2[e])
         y = y.index_add(0, tok, gate[tok, slot, None] * ye)
     return y
+
+
+# ---- attention over packed sequences ------------------------------------------------------------
+def attention_packed(q, k, v, cu, causal, scale=None):
+    """q [T, H, D], k, v [T, Hkv, D] -> (o [T, H, D], lse [H, T]): attention inside every sequence, rows
+    ``cu[b] .. cu[b + 1] - 1``, in the type of ``q``; zeros for rows of no sequence."""
+    T, H, D = q.shape
+    rep = H // k.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    o, lse = torch.zeros_like(q), q.new_zeros(H, T)
+    for r0, r1 in zip(cu[:-1], cu[1:]):
+        if r1 <= r0:
+            continue
+        qs = q[r0:r1].transpose(0, 1)
+        ks, vs = (t[r0:r1].transpose(0, 1).repeat_interleave(rep, dim=0) for t in (k, v))
+        s = torch.matmul(qs, ks.transpose(1, 2)) * scale
+        if causal:
+            s = s.masked_fill(~torch.ones(r1 - r0, r1 - r0, dtype=torch.bool).tril(), float("-inf"))
+        lse = lse.index_copy(1, torch.arange(r0, r1), torch.logsumexp(s, dim=-1))
+        o = o.index_copy(0, torch.arange(r0, r1), torch.matmul(torch.softmax(s, dim=-1), vs).transpose(0, 1))
+    return o, lse
+
+
+# ---- routing in general form ---------------------------------------------------------------------
+def moe_route(logits, topk, scoring="softmax", bias=None, n_group=1, topk_group=1, group_score="max", renorm=True,
+              scale=1.0, idx=None):
+    """One token at a time, as the definition reads.  Returns (idx int64 [T, topk] with -1 where no expert is left,
+    gate [T, topk]); differentiable in ``logits``.  ``idx`` forces the selection."""
+    T, E = logits.shape
+    score = torch.softmax(logits, -1) if scoring == "softmax" else torch.sigmoid(logits)
+    score = torch.where(logits == float("-inf"), torch.zeros_like(score), score)
+    if idx is None:
+        idx = torch.full((T, topk), -1, dtype=torch.long)
+        for t in range(T):
+            there = [e for e in range(E) if logits[t, e] != float("-inf")]
+            choice = {e: float(score[t, e] + bias[e]) if bias is not None else float(logits[t, e]) for e in there}
+            if n_group > 1:
+                gs = E // n_group
+                rank = []
+                for g in range(n_group):
+                    own = [e for e in there if e // gs == g]
+                    if group_score == "max":
+                        value = max((choice[e] for e in own), default=float("-inf"))
+                    else:
+                        best = sorted((float(score[t, e] + (bias[e] if bias is not None else 0)) for e in own))[-2:]
+                        value = sum(best) if best else float("-inf")
+                    rank.append((-value, g))
+                kept = {g for _, g in sorted(rank)[:topk_group]}
+                there = [e for e in there if e // gs in kept]
+            order = sorted(there, key=lambda e: (-choice[e], e))[:topk]
+            idx[t, :len(order)] = torch.tensor(order, dtype=torch.long)
+    picked = torch.where(idx >= 0, score.gather(-1, idx.clamp(min=0)), torch.zeros_like(score[:, :1]))
+    if renorm:
+        total = picked.sum(-1, keepdim=True)
+        picked = picked / torch.where(total == 0, torch.ones_like(total), total)
+    return idx, picked * scale
+
+
+# ---- dropout from a counter-based generator --------------------------------------------------------
+def philox4x32_10(counter, key):
+    """Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) of one counter (4 words) under one key (2 words)."""
+    c, k = list(counter), list(key)
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+def dropout_factors(n, p, seed, offset, site):
+    """The factor (0 or 1 / (1 - p')) of each of ``n`` elements, fp64; p' = round(65536 p) / 65536."""
+    border = 65536 if p >= 1 else min(int(p * 65536 + 0.5), 65535)
+    out = torch.zeros((n + 7) // 8 * 8, dtype=torch.float64)
+    for g in range((n + 7) // 8):
+        words = philox4x32_10([g, offset & 0xFFFFFFFF, offset >> 32, site], [seed & 0xFFFFFFFF, seed >> 32])
+        for w, word in enumerate(words):
+            for half in range(2):
+                if (word >> 16 * half & 0xFFFF) >= border:
+                    out[8 * g + 2 * w + half] = 65536 / (65536 - border)
+    return out[:n]

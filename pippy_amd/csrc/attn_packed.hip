@@ -1,0 +1,721 @@
+// Attention over packed sequences of different lengths (forward, and a deterministic backward in two kernels).
+//
+// The rows of all sequences lie one after the other, sequence b in rows cu[b] .. cu[b+1]-1.  Inside a sequence
+//   S = scale q k^T,  P = softmax(S) (causal: over the keys up to the query),  o = P v,  lse = log sum exp S,
+//   dv = P^T do,  dP = do v^T,  dS = P (dP - sum_j P dP),  dq = scale dS k,  dk = scale dS^T q,
+// and nothing reaches from one sequence into another: a block of rows is loaded through a buffer resource that
+// ends with its sequence, so rows past the end read as zeros whatever the memory behind them holds, and rows
+// that belong to no sequence are neither read nor written.
+//
+// Scores are produced transposed, S^T[key][query], so that a lane holds one query column: softmax statistics
+// are per-lane scalars and the probabilities sit in registers as the second product wants its operand.
+//
+// Which work-group takes which block is a plan built on the device once per batch (pp_attn_packed_plan) and
+// shared by all layers and both directions: the blocks of all sequences, the latest blocks first.  Under a
+// causal mask block j of a sequence costs j + 1 steps, so a launch begins with its longest work-groups and
+// fills up with ever shorter ones, however unequal the sequences are.
+#include "attn_tile.h"
+#include <math.h>
+
+namespace pp {
+
+constexpr int kPlanHeader = 4;   // int32: number of blocks of 64 rows, number of blocks of 128 rows, 0, 0
+constexpr int kPlanBins = 2048;  // block indexes from here on count as one length class
+constexpr int kPlanThreads = 1024;
+
+struct PackedArgs {
+    const uint16_t* q; const uint16_t* k; const uint16_t* v;
+    uint16_t* o; float* lse;
+    const uint16_t* d_o;
+    uint16_t* dq; uint16_t* dk; uint16_t* dv;
+    float* delta;
+    int64_t sq, sk, sv, so, sdo, sdq, sdk, sdv;  // elements between consecutive rows
+    int64_t T;
+    int32_t H, G;       // query heads; query heads per key / value head
+    const int32_t* plan;
+    float scale;
+};
+
+__host__ __device__ inline int64_t plan_blocks64(int64_t T, int64_t n_seq) { return T / 64 + n_seq; }
+__host__ __device__ inline int64_t plan_blocks128(int64_t T, int64_t n_seq) { return T / 128 + n_seq; }
+
+// ---- the plan -----------------------------------------------------------------------------------
+// One work-group; a wave takes a sequence at a time, its lanes the blocks.  Counting sort by block index, the
+// highest first; the order inside a class is left to the atomics, since it only says which work-group does
+// what.  Entries: {first row of the sequence, its length, block index, 0}.
+__global__ __launch_bounds__(kPlanThreads) void attn_packed_plan_kernel(const int32_t* __restrict__ cu, int n_seq,
+                                                                        int T, int32_t* __restrict__ plan,
+                                                                        int cap64, int cap128) {
+    __shared__ int cursor[kPlanBins];
+    __shared__ int part[kPlanThreads];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int kWaves = kPlanThreads / 64;
+    int4* entries = reinterpret_cast<int4*>(plan + kPlanHeader);
+    for (int pass = 0; pass < 2; ++pass) {
+        const int block = pass == 0 ? 64 : 128;
+        const int cap = pass == 0 ? cap64 : cap128;
+        for (int i = tid; i < kPlanBins; i += kPlanThreads) cursor[i] = 0;
+        __syncthreads();
+        for (int place = 0; place < 2; ++place) {
+            for (int b = wave; b < n_seq; b += kWaves) {
+                // bounds that are out of order or out of range make an empty sequence
+                const int r0 = cu[b], r1 = cu[b + 1];
+                const int len = (r0 >= 0 && r1 > r0 && r1 <= T) ? r1 - r0 : 0;
+                const int nb = len / block + (len % block != 0);
+                for (int j = lane; j < nb; j += 64) {
+                    const int bin = j < kPlanBins - 1 ? j : kPlanBins - 1;
+                    const int at = atomicAdd(&cursor[bin], 1);
+                    if (place && at < cap) entries[at] = make_int4(r0, len, j, 0);
+                }
+            }
+            __syncthreads();
+            if (place) break;
+            // counts -> first places: a class begins behind all higher ones (two classes per thread)
+            const int hi = kPlanBins - 1 - 2 * tid, lo = hi - 1;
+            const int n_hi = cursor[hi], n_lo = cursor[lo];
+            part[tid] = n_hi + n_lo;
+            __syncthreads();
+            for (int o = 1; o < kPlanThreads; o <<= 1) {
+                const int add = tid >= o ? part[tid - o] : 0;
+                __syncthreads();
+                part[tid] += add;
+                __syncthreads();
+            }
+            const int begin = part[tid] - n_hi - n_lo;
+            cursor[hi] = begin;
+            cursor[lo] = begin + n_hi;
+            if (tid == kPlanThreads - 1) plan[pass] = part[tid] < cap ? part[tid] : cap;
+            __syncthreads();
+        }
+        entries += cap64;
+    }
+    if (tid < 2) plan[2 + tid] = 0;
+}
+static_assert(kPlanBins == 2 * kPlanThreads, "the scan takes two classes per thread");
+
+// One block of rows of one sequence, and one head, for a work-group.
+struct PackedBlock {
+    int64_t row0;  // first row of the sequence
+    int len, j;    // its length; index of the block inside it
+    int h;
+};
+
+// With a multiple of 8 heads every XCD takes its own heads (keys and values of a head in one L2; the heads of a
+// group that shares them are neighbours), longest block of all its heads first.  Otherwise the blocks are dealt
+// out in order: consecutive work-groups go to different XCDs, and every XCD gets an equal share of each length.
+__device__ __forceinline__ bool packed_block_of(const PackedArgs& a, int heads, const int4* entries, int n_blocks,
+                                                PackedBlock* w) {
+    const uint32_t bid = blockIdx.x;
+    uint32_t t, h;
+    if (heads % 8 == 0) {
+        const uint32_t g = (uint32_t)heads / 8;
+        h = (bid & 7) * g + (bid >> 3) % g;
+        t = (bid >> 3) / g;
+    } else {
+        t = bid / (uint32_t)heads;
+        h = bid % (uint32_t)heads;
+    }
+    if (t >= (uint32_t)n_blocks) return false;
+    const int4 e = entries[t];
+    w->row0 = __builtin_amdgcn_readfirstlane(e.x);
+    w->len = __builtin_amdgcn_readfirstlane(e.y);
+    w->j = __builtin_amdgcn_readfirstlane(e.z);
+    w->h = (int)h;
+    // a plan made for more rows than this call has
+    return w->row0 >= 0 && w->len > 0 && w->row0 + w->len <= a.T;
+}
+
+// Loader of 64-row blocks of a sequence.  Every block gets a resource of its own that begins at the block (so
+// 32-bit offsets suffice however long the sequence is) and ends with the sequence (rows past it read as zeros).
+template <int DS>
+struct PackedTileLoader {
+    const uint16_t* base;
+    int64_t stride;
+    int len;
+    int voff[2];
+    __device__ __forceinline__ void init(const uint16_t* first, int64_t stride_, int len_, int wave, int lane) {
+        base = first;
+        stride = stride_;
+        len = len_;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = (i * 4 + wave) * 8 + (lane >> 3);
+            voff[i] = row * (int)(stride_ * 2) + (((lane & 7) ^ swz_attn(row)) << 4);
+        }
+    }
+    __device__ __forceinline__ void load(uint16_t* lds, int row0, int wave, int64_t extra = 0) const {
+        const int left = len - row0;
+        const __amdgpu_buffer_rsrc_t rsrc =
+            make_rsrc(base + (int64_t)row0 * stride + extra, (uint64_t)(left < 64 ? left : 64) * (uint64_t)stride * 2);
+#pragma unroll
+        for (int s = 0; s < DS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                load_to_lds_b128(rsrc, lds + s * kTile + (i * 4 + wave) * 512, voff[i] + s * 128, 0);
+    }
+};
+
+// ---- forward ------------------------------------------------------------------------------------
+// A work-group owns 64 query rows of one head and walks the keys in blocks of 64.  Its 4 waves are 2 groups of
+// 32 queries x 2 halves of every key block; the two waves of a group merge once, through LDS.
+template <int D, bool CAUSAL>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(const PackedArgs a) {
+    constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
+    constexpr int kOperand = DS * kTile, kStage = 2 * kOperand;
+    uint16_t* const lds = attn_lds;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave & 1, half = wave >> 1;
+    const int l32 = lane & 31, lh = lane >> 5;
+    PackedBlock w;
+    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader), a.plan[0], &w)) return;
+    const int q0 = w.j * 64, qw0 = q0 + 32 * grp, qi = qw0 + l32;
+    const int hk = w.h / a.G;
+
+    PackedTileLoader<DS> lk, lv;
+    lk.init(a.k + w.row0 * a.sk + (int64_t)hk * D, a.sk, w.len, wave, lane);
+    lv.init(a.v + w.row0 * a.sv + (int64_t)hk * D, a.sv, w.len, wave, lane);
+    const int n_blocks = CAUSAL ? w.j + 1 : (w.len + 63) / 64;
+    auto issue = [&](int stage, int j) {
+        lk.load(lds + stage * kStage, j * 64, wave);
+        lv.load(lds + stage * kStage + kOperand, j * 64, wave);
+    };
+
+    // a query past the end computes with the last row and is not stored
+    const int qr = qi < w.len ? qi : w.len - 1;
+    const uint16_t* qp = a.q + (w.row0 + qr) * a.sq + (int64_t)w.h * D;
+    bf16x8_t qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * ks + 8 * lh);
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t)
+        if (t < n_blocks) issue(t, t);
+
+    f32x16_t oacc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[t][e] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;  // l_run: this lane's share of the row sum
+    const float c = a.scale * kLog2e;
+    const int partner = (lane ^ 32) << 2;
+
+    int stage = 0;
+    for (int j = 0; j < n_blocks; ++j) {
+        const int kt0 = j * 64 + 32 * half;
+        await_block<4 * DS, NS>(j, n_blocks);
+        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
+        const uint16_t* Ks = lds + stage * kStage;
+        const uint16_t* Vs = Ks + kOperand;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        if (kt0 >= w.len || (CAUSAL && kt0 > qw0 + 31)) continue;  // no key of this half is seen
+        f32x16_t sacc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8_t kf = read_row_frag(Ks + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], sacc, 0, 0, 0);
+        }
+        // sacc[v]: key kt0 + 8 (v / 4) + 4 lh + v % 4, query qi.  Keys past the last visible one are masked;
+        // wave-uniform: only the diagonal block and the end of the sequence pay for it.
+        const int last = CAUSAL ? (qr < w.len - 1 ? qr : w.len - 1) : w.len - 1;
+        if (kt0 + 31 > (CAUSAL ? qw0 : w.len - 1) || kt0 + 31 >= w.len) {
+            const int lim = last - kt0 - 4 * lh;
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (8 * (v >> 2) + (v & 3) > lim) sacc[v] = -INFINITY;
+        }
+        float mloc = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mloc = fmaxf(mloc, sacc[v]);
+        // the reference maximum only keeps the exponentials in range: it moves when a row exceeds it by 2^8
+        if (__ballot(mloc * c > m_run * c + 8.0f)) {
+            mloc = fmaxf(mloc, __int_as_float(__builtin_amdgcn_ds_bpermute(partner, __float_as_int(mloc))));
+            const float m_new = fmaxf(m_run, mloc);
+            const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m_run - m_new) * c);
+            l_run *= alpha;
+            m_run = m_new;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[t][e] *= alpha;
+        }
+        const float mc = (m_run == -INFINITY ? 0.f : m_run) * c;
+        float psum = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            sacc[v] = __builtin_amdgcn_exp2f(fmaf(sacc[v], c, -mc));
+            psum += sacc[v];
+        }
+        l_run += psum;
+#pragma unroll
+        for (int gp = 0; gp < 2; ++gp) {
+            float pv[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pv[e] = sacc[8 * gp + e];
+            const bf16x8_t pb = pack8(pv);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const bf16x8_t vf = read_col_frag(Vs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, oacc[dt], 0, 0, 0);
+            }
+        }
+    }
+    l_run += __int_as_float(__builtin_amdgcn_ds_bpermute(partner, __float_as_int(l_run)));
+
+    // merge the two halves in a fixed order: [grp][16 DT + 2 values][64 lanes] floats
+    wait_lds();
+    __syncthreads();
+    float* xs = reinterpret_cast<float*>(lds) + grp * ((16 * DT + 2) * 64) + lane;
+    if (half == 1) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) xs[(16 * dt + e) * 64] = oacc[dt][e];
+        xs[16 * DT * 64] = m_run;
+        xs[(16 * DT + 1) * 64] = l_run;
+    }
+    __syncthreads();
+    if (half == 1 || qi >= w.len) return;
+    const float m1 = xs[16 * DT * 64], l1 = xs[(16 * DT + 1) * 64];
+    const float m = fmaxf(m_run, m1);
+    const float a0 = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m) * c);
+    const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m1 - m) * c);
+    const float l = l_run * a0 + l1 * a1, inv_l = 1.0f / l;
+    uint16_t* op = a.o + (w.row0 + qi) * a.so + (int64_t)w.h * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[e] = (oacc[dt][4 * g + e] * a0 + xs[(16 * dt + 4 * g + e) * 64] * a1) * inv_l;
+            const int d = 32 * dt + 8 * g + 4 * lh;
+            *reinterpret_cast<uint2*>(op + d) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+        }
+    if (lh == 0) a.lse[(int64_t)w.h * a.T + w.row0 + qi] = m * a.scale + logf(l);
+}
+
+// ---- backward: dQ -------------------------------------------------------------------------------
+// A work-group owns 64 query rows (2 groups of 32 queries x 2 halves of every key block) and hands the dK / dV
+// kernel the row sums D = sum_j P dP.
+template <int D, bool CAUSAL>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kernel(const PackedArgs a) {
+    constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
+    constexpr int kOperand = DS * kTile, kStage = 2 * kOperand;
+    uint16_t* const lds = attn_lds;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave & 1, half = wave >> 1;
+    const int l32 = lane & 31, lh = lane >> 5;
+    PackedBlock w;
+    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader), a.plan[0], &w)) return;
+    const int q0 = w.j * 64, qw0 = q0 + 32 * grp, qi = qw0 + l32;
+    const int hk = w.h / a.G;
+
+    PackedTileLoader<DS> lk, lv;
+    lk.init(a.k + w.row0 * a.sk + (int64_t)hk * D, a.sk, w.len, wave, lane);
+    lv.init(a.v + w.row0 * a.sv + (int64_t)hk * D, a.sv, w.len, wave, lane);
+    const int n_blocks = CAUSAL ? w.j + 1 : (w.len + 63) / 64;
+    auto issue = [&](int stage, int j) {
+        lk.load(lds + stage * kStage, j * 64, wave);
+        lv.load(lds + stage * kStage + kOperand, j * 64, wave);
+    };
+
+    const int64_t row = w.row0 + (qi < w.len ? qi : w.len - 1);
+    const uint16_t* qp = a.q + row * a.sq + (int64_t)w.h * D;
+    const uint16_t* dop = a.d_o + row * a.sdo + (int64_t)w.h * D;
+    const uint16_t* op = a.o + row * a.so + (int64_t)w.h * D;
+    bf16x8_t qf[KS], dof[KS];
+    // delta = rowsum(dO * O): the lane pair (lh = 0, 1) holds the row
+    float delta_q = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * ks + 8 * lh);
+        dof[ks] = *reinterpret_cast<const bf16x8_t*>(dop + 16 * ks + 8 * lh);
+        Frag x, y;
+        x.v = dof[ks];
+        y.u = *reinterpret_cast<const uint4*>(op + 16 * ks + 8 * lh);
+        delta_q += bf16lo(x.u.x) * bf16lo(y.u.x) + bf16hi(x.u.x) * bf16hi(y.u.x) +
+                   bf16lo(x.u.y) * bf16lo(y.u.y) + bf16hi(x.u.y) * bf16hi(y.u.y) +
+                   bf16lo(x.u.z) * bf16lo(y.u.z) + bf16hi(x.u.z) * bf16hi(y.u.z) +
+                   bf16lo(x.u.w) * bf16lo(y.u.w) + bf16hi(x.u.w) * bf16hi(y.u.w);
+    }
+    delta_q += __shfl_xor(delta_q, 32, 64);
+    const float lse_q = a.lse[(int64_t)w.h * a.T + row] * kLog2e;
+    // The sum of P dP over the keys equals delta in exact arithmetic and is the one under which the rows of dS
+    // sum to zero; it is complete only behind the loop and is what the dK / dV kernel gets.
+    float d_sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t)
+        if (t < n_blocks) issue(t, t);
+    const float c = a.scale * kLog2e;
+
+    f32x16_t dqacc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dqacc[t][e] = 0.f;
+
+    int stage = 0;
+    for (int j = 0; j < n_blocks; ++j) {
+        const int kt0 = j * 64 + 32 * half;
+        await_block<4 * DS, NS>(j, n_blocks);
+        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
+        const uint16_t* Ks = lds + stage * kStage;
+        const uint16_t* Vs = Ks + kOperand;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        if (kt0 >= w.len || (CAUSAL && kt0 > qw0 + 31)) continue;
+        f32x16_t sacc, dpacc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sacc[e] = 0.f;
+            dpacc[e] = 0.f;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8_t kfr = read_row_frag(Ks + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t vfr = read_row_frag(Vs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr, qf[ks], sacc, 0, 0, 0);
+            dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr, dof[ks], dpacc, 0, 0, 0);
+        }
+        float dsv[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) dsv[v] = __builtin_amdgcn_exp2f(fmaf(sacc[v], c, -lse_q));
+        if ((CAUSAL && kt0 + 31 > qw0) || kt0 + 31 >= w.len) {
+            const int last = CAUSAL && qi < w.len - 1 ? qi : w.len - 1;
+            const int lim = last - kt0 - 4 * lh;
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (8 * (v >> 2) + (v & 3) > lim) dsv[v] = 0.f;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) d_sum = fmaf(dsv[v], dpacc[v], d_sum);
+#pragma unroll
+        for (int v = 0; v < 16; ++v) dsv[v] *= dpacc[v] - delta_q;
+#pragma unroll
+        for (int gp = 0; gp < 2; ++gp) {
+            const bf16x8_t dsb = pack8(dsv + 8 * gp);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const bf16x8_t ktf = read_col_frag(Ks + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                dqacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktf, dsb, dqacc[dt], 0, 0, 0);
+            }
+        }
+    }
+    d_sum += __shfl_xor(d_sum, 32, 64);
+    // add the sums of the two halves: [grp][16 DT + 1 values][64 lanes] floats
+    wait_lds();
+    __syncthreads();
+    float* xs = reinterpret_cast<float*>(lds) + grp * ((16 * DT + 1) * 64) + lane;
+    if (half == 1) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) xs[(16 * dt + e) * 64] = dqacc[dt][e];
+        xs[16 * DT * 64] = d_sum;
+    }
+    __syncthreads();
+    if (half == 1 || qi >= w.len) return;
+    d_sum += xs[16 * DT * 64];
+    if (lh == 0) a.delta[(int64_t)w.h * a.T + row] = d_sum;
+    uint16_t* dqp = a.dq + row * a.sdq + (int64_t)w.h * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float s[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = (dqacc[dt][4 * g + e] + xs[(16 * dt + 4 * g + e) * 64]) * a.scale;
+            const int d = 32 * dt + 8 * g + 4 * lh;
+            *reinterpret_cast<uint2*>(dqp + d) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+        }
+}
+
+// ---- backward: dK, dV ---------------------------------------------------------------------------
+// A work-group owns 64 keys of one key / value head and walks the query blocks that see them, one query head of
+// the group after the other, so the sums over a group have a fixed order.  4 waves: 2 groups of 32 keys x 2
+// halves of every query block.
+template <int D, bool CAUSAL>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void attn_packed_bwd_dkv_kernel(const PackedArgs a) {
+    constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
+    constexpr int kOperand = DS * kTile;
+    constexpr int kStage = 2 * kOperand + 256;  // Q, dO, 64 lse, 64 delta
+    uint16_t* const lds = attn_lds;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave & 1, half = wave >> 1;
+    const int l32 = lane & 31, lh = lane >> 5;
+    PackedBlock w;  // w.h: key / value head
+    if (!packed_block_of(a, a.H / a.G, reinterpret_cast<const int4*>(a.plan + kPlanHeader), a.plan[0], &w)) return;
+    const int nbq = (w.len + 63) / 64;
+    // the plan's order is by query work; a key block sees the most queries where a query block sees the fewest
+    // keys, so the block index counts from the end here
+    const int jk = CAUSAL ? nbq - 1 - w.j : w.j;
+    const int kv0 = jk * 64, kvw0 = kv0 + 32 * grp, kvi = kvw0 + l32;
+    const int h0 = w.h * a.G;
+
+    PackedTileLoader<DS> lq, ldo;
+    lq.init(a.q + w.row0 * a.sq + (int64_t)h0 * D, a.sq, w.len, wave, lane);
+    ldo.init(a.d_o + w.row0 * a.sdo + (int64_t)h0 * D, a.sdo, w.len, wave, lane);
+    // waves 0 and 2 fetch lse, waves 1 and 3 delta (the same values twice: every wave issues the same number
+    // of loads, which keeps the outstanding-load arithmetic uniform)
+    const float* stat = ((wave & 1) ? a.delta : a.lse) + (int64_t)h0 * a.T + w.row0;
+    const int stat_off = 2 * kOperand + ((wave & 1) ? 128 : 0);
+
+    const int jq0 = CAUSAL ? jk : 0;
+    const int nb_head = nbq - jq0, nb = a.G * nb_head;
+    int iss_g = 0, iss_b = 0;
+    auto issue = [&](int stage) {  // steps are issued in order
+        uint16_t* st = lds + stage * kStage;
+        const int row0 = (jq0 + iss_b) * 64;
+        lq.load(st, row0, wave, (int64_t)iss_g * D);
+        ldo.load(st + kOperand, row0, wave, (int64_t)iss_g * D);
+        const int left = w.len - row0;
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(stat + (int64_t)iss_g * a.T + row0, (uint64_t)(left < 64 ? left : 64) * 4);
+        load_floats_to_lds(rs, reinterpret_cast<float*>(st + stat_off), 0, lane);
+        if (++iss_b == nb_head) {
+            iss_b = 0;
+            ++iss_g;
+        }
+    };
+
+    const int64_t krow = w.row0 + (kvi < w.len ? kvi : w.len - 1);
+    const uint16_t* kp = a.k + krow * a.sk + (int64_t)w.h * D;
+    const uint16_t* vp = a.v + krow * a.sv + (int64_t)w.h * D;
+    bf16x8_t kf[KS], vf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        kf[ks] = *reinterpret_cast<const bf16x8_t*>(kp + 16 * ks + 8 * lh);
+        vf[ks] = *reinterpret_cast<const bf16x8_t*>(vp + 16 * ks + 8 * lh);
+    }
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t)
+        if (t < nb) issue(t);
+
+    f32x16_t dvacc[DT], dkacc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            dvacc[t][e] = 0.f;
+            dkacc[t][e] = 0.f;
+        }
+    const float c = a.scale * kLog2e;
+
+    int stage = 0, cur_b = 0;
+    for (int j = 0; j < nb; ++j) {
+        const int qt0 = (jq0 + cur_b) * 64 + 32 * half;
+        cur_b = cur_b + 1 == nb_head ? 0 : cur_b + 1;
+        await_block<4 * DS + 1, NS>(j, nb);
+        if (j + NS - 1 < nb) issue(stage == 0 ? NS - 1 : stage - 1);
+        const uint16_t* Qs = lds + stage * kStage;
+        const uint16_t* Os = Qs + kOperand;
+        const float* lse_s = reinterpret_cast<const float*>(Qs + 2 * kOperand);
+        const float* delta_s = lse_s + 64;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        if (qt0 >= w.len || (CAUSAL && qt0 + 31 < kvw0)) continue;  // every query precedes every key
+        f32x16_t sacc, dpacc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sacc[e] = 0.f;
+            dpacc[e] = 0.f;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8_t qfr = read_row_frag(Qs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t ofr = read_row_frag(Os + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qfr, kf[ks], sacc, 0, 0, 0);
+            dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ofr, vf[ks], dpacc, 0, 0, 0);
+        }
+        // element v: query qt0 + 8 (v / 4) + 4 lh + v % 4, key kvi.  A query past the end has zero rows, a zero
+        // log-sum-exp and a zero delta: P = 1 meets dO = 0, dS = 0.
+        float pv[16], dsv[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 l4 = *reinterpret_cast<const float4*>(lse_s + 32 * half + 8 * g + 4 * lh);
+            const float lq4[4] = {l4.x * kLog2e, l4.y * kLog2e, l4.z * kLog2e, l4.w * kLog2e};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                pv[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sacc[4 * g + e], c, -lq4[e]));
+        }
+        if (CAUSAL && qt0 < kvw0 + 31) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (kvi > qt0 + 8 * (v >> 2) + 4 * lh + (v & 3)) pv[v] = 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 d4 = *reinterpret_cast<const float4*>(delta_s + 32 * half + 8 * g + 4 * lh);
+            const float dq4[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dsv[4 * g + e] = pv[4 * g + e] * (dpacc[4 * g + e] - dq4[e]);
+        }
+#pragma unroll
+        for (int gp = 0; gp < 2; ++gp) {
+            const bf16x8_t pb = pack8(pv + 8 * gp);
+            const bf16x8_t dsb = pack8(dsv + 8 * gp);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const bf16x8_t otf = read_col_frag(Os + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t qtf = read_col_frag(Qs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                dvacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(otf, pb, dvacc[dt], 0, 0, 0);
+                dkacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtf, dsb, dkacc[dt], 0, 0, 0);
+            }
+        }
+    }
+    // add the sums of the two halves: [grp][16 DT values][64 lanes] floats, dV then dK
+    wait_lds();
+    __syncthreads();
+    float* xs = reinterpret_cast<float*>(lds) + grp * (16 * DT * 64) + lane;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+        f32x16_t(&acc)[DT] = pass == 0 ? dvacc : dkacc;
+        if (half == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) xs[(16 * dt + e) * 64] = acc[dt][e];
+        }
+        __syncthreads();
+        if (half == 0 && kvi < w.len) {
+            uint16_t* outp = (pass == 0 ? a.dv + krow * a.sdv : a.dk + krow * a.sdk) + (int64_t)w.h * D;
+            const float f = pass == 0 ? 1.0f : a.scale;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float s[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[e] = (acc[dt][4 * g + e] + xs[(16 * dt + 4 * g + e) * 64]) * f;
+                    const int d = 32 * dt + 8 * g + 4 * lh;
+                    *reinterpret_cast<uint2*>(outp + d) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+                }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- entry points -------------------------------------------------------------------------------
+static int packed_check(const char* who, const pp_attn_packed_desc* d, bool bwd) {
+    if (!d) return fail(PP_ERR_INVALID, "%s: null descriptor", who);
+    if (d->T < 0 || d->T > 0x7fffffc0ll || d->n_seq < 0 || d->n_seq > 0x7fffffc0ll || d->H <= 0 || d->Hkv <= 0 ||
+        d->H % d->Hkv)
+        return fail(PP_ERR_INVALID, "%s: bad shape (T=%lld n_seq=%lld H=%lld Hkv=%lld)", who, (long long)d->T,
+                    (long long)d->n_seq, (long long)d->H, (long long)d->Hkv);
+    if (d->D != 64 && d->D != 128)
+        return fail(PP_ERR_UNSUPPORTED, "%s: head_dim %lld (64 and 128 are built)", who, (long long)d->D);
+    if (!(d->scale > 0.f) || !(d->scale < INFINITY))
+        return fail(PP_ERR_INVALID, "%s: scale must be positive and finite", who);
+    const struct { const void* p; int64_t stride, width; const char* name; bool need; } rows[] = {
+        {d->q, d->stride_q, d->H * d->D, "q", true},     {d->k, d->stride_k, d->Hkv * d->D, "k", true},
+        {d->v, d->stride_v, d->Hkv * d->D, "v", true},   {d->o, d->stride_o, d->H * d->D, "o", true},
+        {d->d_o, d->stride_do, d->H * d->D, "d_o", bwd}, {d->dq, d->stride_dq, d->H * d->D, "dq", bwd},
+        {d->dk, d->stride_dk, d->Hkv * d->D, "dk", bwd}, {d->dv, d->stride_dv, d->Hkv * d->D, "dv", bwd}};
+    for (const auto& r : rows) {
+        if (!r.need) continue;
+        if (!r.p || !aligned(r.p, 16)) return fail(PP_ERR_INVALID, "%s: %s must be a 16-byte aligned pointer", who, r.name);
+        // 64 rows of a block are addressed with 32-bit byte offsets
+        if (r.stride % 8 || r.stride < r.width || r.stride > (1 << 23))
+            return fail(PP_ERR_INVALID, "%s: row stride %lld of %s must be a multiple of 8 in [%lld, %d]", who,
+                        (long long)r.stride, r.name, (long long)r.width, 1 << 23);
+    }
+    if (!d->lse || !d->plan || !aligned(d->plan, 16) || (bwd && !d->delta))
+        return fail(PP_ERR_INVALID, "%s: null pointer, or a plan that is not 16-byte aligned", who);
+    if (plan_blocks64(d->T, d->n_seq) * d->H > 0x7fffff00ll) return fail(PP_ERR_UNSUPPORTED, "%s: grid too large", who);
+    return PP_OK;
+}
+
+static PackedArgs packed_args(const pp_attn_packed_desc* d) {
+    PackedArgs a;
+    a.q = (const uint16_t*)d->q; a.k = (const uint16_t*)d->k; a.v = (const uint16_t*)d->v;
+    a.o = (uint16_t*)d->o; a.lse = d->lse;
+    a.d_o = (const uint16_t*)d->d_o;
+    a.dq = (uint16_t*)d->dq; a.dk = (uint16_t*)d->dk; a.dv = (uint16_t*)d->dv;
+    a.delta = d->delta;
+    a.sq = d->stride_q; a.sk = d->stride_k; a.sv = d->stride_v; a.so = d->stride_o;
+    a.sdo = d->stride_do; a.sdq = d->stride_dq; a.sdk = d->stride_dk; a.sdv = d->stride_dv;
+    a.T = d->T;
+    a.H = (int32_t)d->H;
+    a.G = (int32_t)(d->H / d->Hkv);
+    a.plan = d->plan;
+    a.scale = d->scale;
+    return a;
+}
+
+// Dynamic LDS: the stages, or the exchange buffers of the epilogue if those are larger.
+static size_t packed_lds_bytes(int D, bool dkv) {
+    const size_t stages = (size_t)attn_stages(D) * ((size_t)2 * (D / 64) * kTile * 2 + (dkv ? 512 : 0));
+    const size_t merge = (size_t)2 * (16 * (D / 32) + 2) * 64 * 4;
+    return stages > merge ? stages : merge;
+}
+
+template <auto kernel>
+static int packed_launch(const char* name, int64_t grid, size_t lds, hipStream_t st, const PackedArgs& a) {
+    static const hipError_t attr_rc =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (attr_rc != hipSuccess)
+        return fail(PP_ERR_LAUNCH, "%s: cannot reserve %zu bytes of LDS: %s", name, lds, hipGetErrorString(attr_rc));
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(256), lds, st, a);
+    return check_launch(name);
+}
+
+template <int D, bool CAUSAL>
+static int packed_fwd(const pp_attn_packed_desc* d, hipStream_t st) {
+    return packed_launch<attn_packed_fwd_kernel<D, CAUSAL>>("attn_packed_fwd_kernel", plan_blocks64(d->T, d->n_seq) * d->H,
+                                                            packed_lds_bytes(D, false), st, packed_args(d));
+}
+
+template <int D, bool CAUSAL>
+static int packed_bwd(const pp_attn_packed_desc* d, hipStream_t st) {
+    const PackedArgs a = packed_args(d);
+    const int64_t blocks = plan_blocks64(d->T, d->n_seq);
+    // the dQ kernel goes first: it leaves the row sums that the dK / dV kernel reads
+    const int rc = packed_launch<attn_packed_bwd_dq_kernel<D, CAUSAL>>("attn_packed_bwd_dq_kernel", blocks * d->H,
+                                                                       packed_lds_bytes(D, false), st, a);
+    if (rc) return rc;
+    return packed_launch<attn_packed_bwd_dkv_kernel<D, CAUSAL>>("attn_packed_bwd_dkv_kernel", blocks * d->Hkv,
+                                                                packed_lds_bytes(D, true), st, a);
+}
+
+}  // namespace pp
+
+using namespace pp;
+
+extern "C" int64_t pp_attn_packed_plan_ints(int64_t n_seq, int64_t T) {
+    if (n_seq < 0 || T < 0 || n_seq > 0x7fffffc0ll || T > 0x7fffffc0ll) return -1;
+    return kPlanHeader + 4 * (plan_blocks64(T, n_seq) + plan_blocks128(T, n_seq));
+}
+
+extern "C" int pp_attn_packed_plan(const int32_t* cu_seqlens, int64_t n_seq, int64_t T, int32_t* plan, pp_stream stream) {
+    if (pp_attn_packed_plan_ints(n_seq, T) < 0 || plan_blocks64(T, n_seq) > 0x7fffffc0ll)
+        return fail(PP_ERR_INVALID, "pp_attn_packed_plan: bad shape (n_seq=%lld T=%lld)", (long long)n_seq, (long long)T);
+    if (!plan || !aligned(plan, 16) || (n_seq > 0 && !cu_seqlens))
+        return fail(PP_ERR_INVALID, "pp_attn_packed_plan: null pointer, or a plan that is not 16-byte aligned");
+    hipLaunchKernelGGL(attn_packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream),
+                       cu_seqlens, (int)n_seq, (int)T, plan, (int)plan_blocks64(T, n_seq), (int)plan_blocks128(T, n_seq));
+    return check_launch("attn_packed_plan_kernel");
+}
+
+extern "C" int pp_attn_packed_fwd(const pp_attn_packed_desc* d, pp_stream stream) {
+    const int rc = packed_check("pp_attn_packed_fwd", d, false);
+    if (rc) return rc;
+    if (d->T == 0 || d->n_seq == 0) return PP_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (d->D == 64) return d->causal ? packed_fwd<64, true>(d, st) : packed_fwd<64, false>(d, st);
+    return d->causal ? packed_fwd<128, true>(d, st) : packed_fwd<128, false>(d, st);
+}
+
+extern "C" int pp_attn_packed_bwd(const pp_attn_packed_desc* d, pp_stream stream) {
+    const int rc = packed_check("pp_attn_packed_bwd", d, true);
+    if (rc) return rc;
+    if (d->T == 0 || d->n_seq == 0) return PP_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (d->D == 64) return d->causal ? packed_bwd<64, true>(d, st) : packed_bwd<64, false>(d, st);
+    return d->causal ? packed_bwd<128, true>(d, st) : packed_bwd<128, false>(d, st);
+}
