@@ -46,30 +46,111 @@ __device__ __forceinline__ void dropout_factors(const DropoutArgs& a, uint64_t s
     }
 }
 
+// A dropped element contributes a zero whatever it holds (an infinity or NaN too).  In bf16 the work is one 16-byte
+// access per tensor and group; FLAT: one row, whose elements are addressed without a division.
 template <typename ET>
-__device__ __forceinline__ float dropout_load(const void* p, int64_t i) {
-    if constexpr (sizeof(ET) == 2) return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
-    else return static_cast<const float*>(p)[i];
-}
+struct DropoutVec;
+template <>
+struct DropoutVec<uint16_t> {
+    uint4 w;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+        v[0] = bf16lo(w.x); v[1] = bf16hi(w.x); v[2] = bf16lo(w.y); v[3] = bf16hi(w.y);
+        v[4] = bf16lo(w.z); v[5] = bf16hi(w.z); v[6] = bf16lo(w.w); v[7] = bf16hi(w.w);
+    }
+    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&v)[8]) {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+    static __device__ __forceinline__ float load1(const void* p, int64_t i) {
+        return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
+    }
+    static __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
+        static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
+    }
+};
+template <>
+struct DropoutVec<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        a = q[0];
+        b = q[1];
+    }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    static __device__ __forceinline__ void store(void* p, int64_t i, const float (&v)[8]) {
+        float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+        q[0] = make_float4(v[0], v[1], v[2], v[3]);
+        q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    static __device__ __forceinline__ float load1(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
+    static __device__ __forceinline__ void store1(void* p, int64_t i, float v) { static_cast<float*>(p)[i] = v; }
+};
 
-// A dropped element contributes a zero whatever it holds (an infinity or NaN too).
-template <typename ET>
+constexpr int kDropoutGroups = 2;  // groups of 8 elements per lane: their loads are all in flight at once
+
+template <typename ET, bool FLAT, bool RESID>
 __global__ __launch_bounds__(256) void dropout_kernel(const DropoutArgs a) {
     const uint64_t seed = a.rng[0], offset = a.rng[1];
-    const int64_t per_row = (a.C + 7) / 8, n = a.rows * per_row;
-    for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < n; g += (int64_t)gridDim.x * 256) {
+    const uint32_t per_row = (uint32_t)((a.C + 7) / 8);
+    const uint64_t n = (uint64_t)a.rows * (uint64_t)((a.C + 7) / 8), n_whole = FLAT ? (uint64_t)a.C / 8 : n;
+    const uint64_t g0 = (uint64_t)blockIdx.x * (256 * kDropoutGroups) + threadIdx.x;
+    DropoutVec<ET> x[kDropoutGroups], r[kDropoutGroups];
+    uint32_t row[kDropoutGroups], col[kDropoutGroups];
+#pragma unroll
+    for (int q = 0; q < kDropoutGroups; ++q) {
+        const uint64_t g = g0 + q * 256;
+        row[q] = 0;
+        col[q] = 0;
+        if (g >= n_whole) continue;
+        if constexpr (!FLAT) {
+            row[q] = (uint32_t)g / per_row;  // fewer than 2^32 groups
+            col[q] = (uint32_t)g % per_row;
+        }
+        x[q].load(a.x, FLAT ? (int64_t)g * 8 : row[q] * a.ld_x + (int64_t)col[q] * 8);
+        if constexpr (RESID) r[q].load(a.resid, FLAT ? (int64_t)g * 8 : row[q] * a.ld_r + (int64_t)col[q] * 8);
+    }
+#pragma unroll
+    for (int q = 0; q < kDropoutGroups; ++q) {
+        const uint64_t g = g0 + q * 256;
+        if (g >= n) continue;
         float f[8];
         dropout_factors(a, seed, offset, (uint32_t)g, f);
-        const int64_t r = g / per_row, c0 = (g % per_row) * 8;
+        if (g < n_whole) {
+            float v[8], t[8], y[8];
+            x[q].unpack(v);
+            if constexpr (RESID) r[q].unpack(t);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (c0 + e >= a.C) break;
-            float v = a.resid ? dropout_load<ET>(a.resid, r * a.ld_r + c0 + e) : 0.f;
-            if (f[e] != 0.f) v = fmaf(dropout_load<ET>(a.x, r * a.ld_x + c0 + e), f[e], v);
-            if constexpr (sizeof(ET) == 2) static_cast<uint16_t*>(a.y)[r * a.ld_y + c0 + e] = f32_to_bf16(v);
-            else static_cast<float*>(a.y)[r * a.ld_y + c0 + e] = v;
+            for (int e = 0; e < 8; ++e) {
+                const float kept = f[e] != 0.f ? v[e] : 0.f;
+                y[e] = RESID ? fmaf(kept, f[e], t[e]) : kept * f[e];
+            }
+            DropoutVec<ET>::store(a.y, FLAT ? (int64_t)g * 8 : row[q] * a.ld_y + (int64_t)col[q] * 8, y);
+        } else {  // the last elements of a flat tensor whose length is no multiple of 8
+            for (int e = 0; e < 8 && (int64_t)g * 8 + e < a.C; ++e) {
+                const int64_t i = (int64_t)g * 8 + e;
+                float v = RESID ? DropoutVec<ET>::load1(a.resid, i) : 0.f;
+                if (f[e] != 0.f) v = fmaf(DropoutVec<ET>::load1(a.x, i), f[e], v);
+                DropoutVec<ET>::store1(a.y, i, v);
+            }
         }
     }
+}
+
+template <typename ET>
+static int dropout_launch(const DropoutArgs& a, hipStream_t st) {
+    const int64_t groups = a.rows * ((a.C + 7) / 8), per_block = 256 * kDropoutGroups;
+    const dim3 grid((unsigned)((groups + per_block - 1) / per_block));
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
+        return check_launch("dropout_kernel");
+    };
+    if (a.rows == 1) return a.resid ? go(dropout_kernel<ET, true, true>) : go(dropout_kernel<ET, true, false>);
+    return a.resid ? go(dropout_kernel<ET, false, true>) : go(dropout_kernel<ET, false, false>);
 }
 
 __global__ void rng_advance_kernel(uint64_t* rng, uint64_t step) { rng[1] += step; }
@@ -96,12 +177,8 @@ static int dropout_run(const char* who, const void* x, int64_t ld_x, const void*
     const uint32_t border = (uint32_t)(p * 65536.0f + 0.5f);
     a.border = p >= 1.f ? 65536u : (border > 65535u ? 65535u : border);
     a.scale = p >= 1.f ? 0.f : 65536.0f / (float)(65536u - a.border);
-    const int64_t blocks = (rows * ((C + 7) / 8) + 255) / 256;
-    const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == PP_BF16) hipLaunchKernelGGL(dropout_kernel<uint16_t>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(dropout_kernel<float>, grid, dim3(256), 0, st, a);
-    return check_launch("dropout_kernel");
+    return dtype == PP_BF16 ? dropout_launch<uint16_t>(a, st) : dropout_launch<float>(a, st);
 }
 
 }  // namespace pp

@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
     }
     // the slots of this token: gradient of the weight and the score, in every lane
     float dg[kRouteMaxK], sk[kRouteMaxK];
-    float total = 0.f, along = 0.f;
+    float total = 0.f;
 #pragma unroll
     for (int k = 0; k < kRouteMaxK; ++k) {
         dg[k] = sk[k] = 0.f;
@@ -269,15 +269,30 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
             if (j * 64 + lane == e) own = s[j];
         sk[k] = __shfl(own, e & 63, 64);
         total += sk[k];
-        along = fmaf(sk[k], dg[k], along);
     }
+    // With renorm the differences are taken against the first slot's gradient (the weights sum to one): a token
+    // with a single expert gets exactly no gradient.  Then sum_j s_j ds_j is zero, and softmax scores pass
+    // nothing on to the experts that were not selected.
     float dot = 0.f;  // sum_j s_j ds_j over the selected experts
+    float along = 0.f;
+    if (a.renorm) {
+        const float ref = dg[0];
+#pragma unroll
+        for (int k = 0; k < kRouteMaxK; ++k) {
+            if (k >= a.K) break;
+            dg[k] -= ref;
+            along = fmaf(sk[k], dg[k], along);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < kRouteMaxK; ++k) {
         if (k >= a.K) break;
-        if (a.renorm) dg[k] = total == 0.f ? 0.f : a.scale * (dg[k] - along / total) / total;
-        else dg[k] *= a.scale;
-        dot = fmaf(sk[k], dg[k], dot);
+        if (a.renorm) {
+            dg[k] = total == 0.f ? 0.f : a.scale * (dg[k] - along / total) / total;
+        } else {
+            dg[k] *= a.scale;
+            dot = fmaf(sk[k], dg[k], dot);
+        }
     }
     float d[V];
 #pragma unroll
