@@ -24,11 +24,19 @@ struct RouteArgs {
     int64_t ld, T;
     const float* bias;
     int32_t E, K, n_group, topk_group;
-    int32_t renorm;
+    int32_t group_top2, renorm;
+    int32_t vec;  // rows of logits are 16-byte aligned
     float scale;
     int32_t* idx;
     float* gate;
 };
+constexpr float kRouteLog2e = 1.44269504088896340736f;
+
+// Orders a wave's LDS accesses with those of its other lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
 template <typename LT>
 __device__ __forceinline__ float route_load(const void* p, int64_t i) {
@@ -36,159 +44,356 @@ __device__ __forceinline__ float route_load(const void* p, int64_t i) {
     else return static_cast<const float*>(p)[i];
 }
 
-// Total order of the choices as unsigned numbers: 0 is "not there", 1 a NaN, then the numbers upwards
-// (-0 counts as 0).
-__device__ __forceinline__ uint64_t route_key(double c) {
+// Total order as unsigned numbers: 0 is "not there", 1 a NaN, then the numbers upwards (-0 counts as 0).
+__device__ __forceinline__ uint32_t route_key(float c) {
     if (c != c) return 1;
-    const uint64_t b = __builtin_bit_cast(uint64_t, c + 0.0);
-    return (b >> 63) ? ~b : (b | (1ull << 63));
+    const uint32_t b = __float_as_uint(c + 0.0f);
+    return (b >> 31) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float route_value(uint32_t key) {  // of a key > 1
+    return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key);
 }
 
-template <int G, typename T>
-__device__ __forceinline__ T group_max(T v) {
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) {
-        const T w = __shfl_xor(v, o, G);
-        v = w > v ? w : v;
-    }
+// Reductions over the G neighbouring lanes of a token; every lane gets the result.  Inside 16 lanes the partners come
+// through DPP (two quad permutations and two mirrors; after a step all lanes of a set hold the same), beyond that
+// through a shuffle.
+template <int CTRL>
+__device__ __forceinline__ uint32_t route_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int G, typename F>
+__device__ __forceinline__ uint32_t route_reduce(uint32_t v, F f) {
+    static_assert(G == 8 || G == 16 || G == 32, "lanes per token");
+    v = f(v, route_dpp<0xB1>(v));   // quad_perm 1 0 3 2
+    v = f(v, route_dpp<0x4E>(v));   // quad_perm 2 3 0 1
+    v = f(v, route_dpp<0x141>(v));  // row_half_mirror
+    if constexpr (G >= 16) v = f(v, route_dpp<0x140>(v));  // row_mirror
+    if constexpr (G >= 32) v = f(v, (uint32_t)__shfl_xor((int)v, 16, 64));
     return v;
 }
 template <int G>
-__device__ __forceinline__ int group_min(int v) {
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, G));
-    return v;
+__device__ __forceinline__ uint32_t route_max(uint32_t v) {
+    return route_reduce<G>(v, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
 }
-template <int G, typename T>
-__device__ __forceinline__ T group_sum(T v) {
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, G);
-    return v;
+template <int G>
+__device__ __forceinline__ uint32_t route_min(uint32_t v) {
+    return route_reduce<G>(v, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+}
+template <int G>
+__device__ __forceinline__ float route_fmax(float v) {
+    return __uint_as_float(route_reduce<G>(__float_as_uint(v), [](uint32_t x, uint32_t y) {
+        return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+    }));
+}
+template <int G>
+__device__ __forceinline__ float route_fsum(float v) {
+    return __uint_as_float(route_reduce<G>(__float_as_uint(v), [](uint32_t x, uint32_t y) {
+        return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+    }));
 }
 
-// G lanes per token, V consecutive experts per lane.  Scores are formed in 64 bits: two choices that differ by
-// less than an fp32 rounding are still told apart.
-template <typename LT, int G, int V, bool SIGMOID, bool TOP2>
+// How far apart two choices formed in fp32 must be for their order to be certain.  A score is off by at most
+//   sigmoid: s (1 - s) (1.5 |x| 2^-24 + 2^-23) from the exponential (|x| s (1 - s) < 0.23), 3 s 2^-24 from the quotient:
+//            below 2^-21;
+//   softmax: s (|x - m| 2^-24 + 2^-23) from the exponential (|x - m| s < 0.37 s_max), s (V + 5 + 4) 2^-24 from the sum and
+//            the quotient: below 2^-19 of the row's largest score for V <= 16;
+// and the sum with the bias by half a step of itself.  The margin is twice that.
+template <bool SIGMOID>
+__device__ __forceinline__ float route_margin(float s_max, float c) {
+    return (SIGMOID ? 0x1p-20f : 0x1p-18f * s_max) + 0x1p-22f * fabsf(c);
+}
+
+// The same values in 64 bits, for the few experts whose order fp32 leaves open.
+template <bool SIGMOID>
+__device__ __forceinline__ double route_score64(float x, float m, double sum) {
+    if constexpr (SIGMOID) return 1.0 / (1.0 + exp(-(double)x));
+    else return exp((double)x - (double)m) / sum;
+}
+template <typename LT, int G>
+__device__ __forceinline__ double route_sum64(const RouteArgs& a, int64_t t, int li, float m) {
+    double sum = 0.0;
+    for (int e = li; e < a.E; e += G) {
+        const float x = route_load<LT>(a.logits, t * a.ld + e);
+        if (x != -INFINITY) sum += exp((double)x - (double)m);
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    return sum;
+}
+
+// G lanes per token, V consecutive experts per lane, V <= 16.  K rounds of: largest key of the lanes, the experts
+// that may hold it, the winner.  Without a bias the keys are the logits, exact, and equal ones go to the lowest
+// index.  With one they are the fp32 choices: the experts within the margin of the largest (nearly always just
+// one) are compared in 64 bits.  The weights are formed from the selected experts' logits alone.
+//
+// Bound by the instructions of the K rounds (about 5 V + 30 each for 64 / G tokens a wave) and, below a few thousand
+// tokens, by latency.  16 lanes of 16 experts for E = 256 make a round four tokens' worth of work per wave; a
+// wave per token spends most of a round on the reductions.
+template <typename LT, int G, int V, bool SIGMOID, bool BIASED>
 __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
-    constexpr int kTokens = 256 / G;
-    __shared__ uint64_t gkey[kTokens][kRouteMaxGroups];
-    __shared__ float picked[kTokens][kRouteMaxK];
-    const int tid = threadIdx.x, li = tid % G, slot = tid / G;
+    constexpr int kTokens = 256 / G, kE = G * V;
+    __shared__ uint32_t gkey[kTokens][kRouteMaxGroups];
+    __shared__ uint32_t ckey[kTokens][kE];
+    __shared__ int chosen[kTokens][kRouteMaxK];
+    const int tid = threadIdx.x, li = tid % G, slot = tid / G, lane = tid & 63;
     const int64_t t0 = (int64_t)blockIdx.x * kTokens + slot;
     const int64_t t = t0 < a.T ? t0 : a.T - 1;
     const int e0 = li * V;
+    const unsigned long long mine = ((1ull << (G & 63)) - 1ull) << (lane & ~(G - 1));  // this token's lanes
 
     float x[V];
-    float m = -INFINITY;
+    constexpr int kVec = 16 / (int)sizeof(LT);
+    bool done = false;
+    if constexpr (V % kVec == 0) {
+        if (a.vec && e0 + V <= a.E) {
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const LT*>(a.logits) + t * a.ld + e0);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        x[j] = e0 + j < a.E ? route_load<LT>(a.logits, t * a.ld + e0 + j) : -INFINITY;
-        m = fmaxf(m, x[j]);
+            for (int i = 0; i < V / kVec; ++i) {
+                const uint4 w = p[i];
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if constexpr (sizeof(LT) == 2) {
+                        x[i * 8 + 2 * q] = bf16lo(u[q]);
+                        x[i * 8 + 2 * q + 1] = bf16hi(u[q]);
+                    } else {
+                        x[i * 4 + q] = __uint_as_float(u[q]);
+                    }
+                }
+            }
+            done = true;
+        }
     }
-    double s[V];
-    if constexpr (SIGMOID) {
+    if (!done) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = 1.0 / (1.0 + exp(-(double)x[j]));
-    } else {
-        m = group_max<G>(m);
-        double sum = 0.0;
+        for (int j = 0; j < V; ++j) x[j] = e0 + j < a.E ? route_load<LT>(a.logits, t * a.ld + e0 + j) : -INFINITY;
+    }
+
+    // scores of all experts in fp32, where anything needs them: the choices of a bias or of sums over groups, or
+    // the sum of softmax weights that are not renormalised
+    const bool top2 = a.n_group > 1 && a.group_top2;
+    float m = -INFINITY, sum = 1.f, s_max = 1.f;
+    float s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = 0.f;
+    if constexpr (SIGMOID) {
+        if (BIASED || top2) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x[j] * kRouteLog2e));
+        }
+    } else if (BIASED || top2 || !a.renorm) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, x[j]);
+        m = route_fmax<G>(m);
+        sum = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            s[j] = x[j] == -INFINITY ? 0.0 : exp((double)x[j] - (double)m);
+            s[j] = x[j] == -INFINITY ? 0.f : expf(x[j] - m);
             sum += s[j];
         }
-        sum = group_sum<G>(sum);
+        sum = route_fsum<G>(sum);
+        s_max = 1.0f / sum;
+        if (BIASED || top2) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[j] /= sum;
+            for (int j = 0; j < V; ++j) s[j] *= s_max;
+        }
     }
-    double c[V];
-    uint64_t key[V];
+    uint32_t key[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const bool there = e0 + j < a.E && x[j] != -INFINITY;
-        c[j] = a.bias && there ? s[j] + (double)a.bias[e0 + j] : s[j];
-        // without a bias the logits rank exactly as the scores do, also where those saturate
-        key[j] = !there ? 0 : route_key(a.bias ? c[j] : (double)x[j]);
+        if constexpr (BIASED) key[j] = there ? route_key(s[j] + a.bias[e0 + j]) : 0;
+        else key[j] = there ? route_key(x[j]) : 0;
     }
+
     if (a.n_group > 1) {
         const int gs = a.E / a.n_group;
-        for (int g = 0; g < a.n_group; ++g) {
-            uint64_t k1 = 0;
-            double b1 = -INFINITY, b2 = -INFINITY;
+        // sums of two rank scores (plus bias); a maximum ranks as the keys themselves do
+        const bool summed = top2;
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if ((e0 + j) / gs == g && key[j] > 1) {
-                    if (key[j] > k1) k1 = key[j];
-                    if (c[j] > b1) {
-                        b2 = b1;
-                        b1 = c[j];
-                    } else if (c[j] > b2) {
-                        b2 = c[j];
-                    }
+        for (int j = 0; j < V; ++j)
+            ckey[slot][e0 + j] = key[j] == 0 ? 0 : (summed && !BIASED ? route_key(s[j]) : key[j]);
+        __syncthreads();
+        const bool open_order = BIASED || summed;  // group scores in fp32 may be out of order
+        for (int g = li; g < a.n_group; g += G) {
+            uint32_t k1 = 0, k2 = 0;
+            for (int e = g * gs; e < (g + 1) * gs; ++e) {
+                const uint32_t k = ckey[slot][e];
+                if (k > k1) {
+                    k2 = k1;
+                    k1 = k;
+                } else if (k > k2) {
+                    k2 = k;
                 }
-            uint64_t k;
-            if constexpr (TOP2) {
-#pragma unroll
-                for (int o = G / 2; o > 0; o >>= 1) {
-                    const double o1 = __shfl_xor(b1, o, G), o2 = __shfl_xor(b2, o, G);
-                    b2 = fmax(fmin(b1, o1), fmax(b2, o2));
-                    b1 = fmax(b1, o1);
-                }
-                // a group with one expert left counts that one
-                k = b1 == -INFINITY ? 0 : route_key(b2 == -INFINITY ? b1 : b1 + b2);
-            } else {
-                k = group_max<G>(k1);
             }
-            if (li == 0) gkey[slot][g] = k;
+            // a group with one expert left counts that one; a NaN counts as not there
+            gkey[slot][g] = !summed ? (k1 > 1 ? k1 : 0) : k1 <= 1 ? 0 : k2 <= 1 ? k1 : route_key(route_value(k1) + route_value(k2));
         }
         __syncthreads();
-        uint64_t open = 0;
-        for (int g = 0; g < a.n_group; ++g) {
-            int ahead = 0;
-            for (int o = 0; o < a.n_group; ++o)
-                ahead += gkey[slot][o] > gkey[slot][g] || (gkey[slot][o] == gkey[slot][g] && o < g);
-            if (ahead < a.topk_group) open |= 1ull << g;
+        unsigned long long open = 0;
+        {
+            uint32_t kept_min = 0xffffffffu, shut_max = 0;
+            for (int g = 0; g < a.n_group; ++g) {
+                const uint32_t own = gkey[slot][g];
+                int ahead = 0;
+                for (int o = li; o < a.n_group; o += G) {
+                    const uint32_t other = gkey[slot][o];
+                    ahead += other > own || (other == own && o < g);
+                }
+                ahead = (int)route_reduce<G>((uint32_t)ahead, [](uint32_t p, uint32_t q) { return p + q; });
+                if (ahead < a.topk_group) {
+                    open |= 1ull << g;
+                    kept_min = own < kept_min ? own : kept_min;
+                } else {
+                    shut_max = own > shut_max ? own : shut_max;
+                }
+            }
+            bool doubt = false;
+            if (open_order && shut_max > 1 && kept_min > 1) {
+                const float hi = route_value(kept_min), lo = route_value(shut_max);
+                doubt = hi - lo <= 2.0f * route_margin<SIGMOID>(s_max, fmaxf(fabsf(hi), fabsf(lo)));
+            }
+            // (the threshold of a group's two best members is below: their own margins count too)
+            if (__any(doubt)) {
+                // the group scores again in 64 bits, from the members that may be the two largest
+                const double total = SIGMOID ? 1.0 : route_sum64<LT, G>(a, t, li, m);
+                __shared__ double wide[kTokens][kRouteMaxGroups];
+                for (int g = li; g < a.n_group; g += G) {
+                    uint32_t k1 = 0, k2 = 0;
+                    for (int e = g * gs; e < (g + 1) * gs; ++e) {
+                        const uint32_t k = ckey[slot][e];
+                        if (k > k1) {
+                            k2 = k1;
+                            k1 = k;
+                        } else if (k > k2) {
+                            k2 = k;
+                        }
+                    }
+                    const uint32_t least = summed && k2 > 1 ? k2 : k1;
+                    double b1 = -INFINITY, b2 = -INFINITY;
+                    if (k1 > 1) {
+                        const float v = route_value(least);
+                        const uint32_t from = route_key(v - route_margin<SIGMOID>(s_max, v));
+                        for (int e = g * gs; e < (g + 1) * gs; ++e) {
+                            if (ckey[slot][e] <= 1 || ckey[slot][e] < from) continue;
+                            double c = route_score64<SIGMOID>(route_load<LT>(a.logits, t * a.ld + e), m, total);
+                            if constexpr (BIASED) c += (double)a.bias[e];
+                            if (c > b1) {
+                                b2 = b1;
+                                b1 = c;
+                            } else if (c > b2) {
+                                b2 = c;
+                            }
+                        }
+                    }
+                    wide[slot][g] = !summed || b2 == -INFINITY ? b1 : b1 + b2;
+                }
+                wave_lds_fence();
+                unsigned long long again = 0;
+                for (int g = 0; g < a.n_group; ++g) {
+                    const double own = wide[slot][g];
+                    int ahead = 0;
+                    for (int o = 0; o < a.n_group; ++o) ahead += wide[slot][o] > own || (wide[slot][o] == own && o < g);
+                    if (ahead < a.topk_group) again |= 1ull << g;
+                }
+                if (doubt) open = again;
+            }
         }
 #pragma unroll
         for (int j = 0; j < V; ++j)
             if (e0 + j < a.E && !((open >> ((e0 + j) / gs)) & 1)) key[j] = 0;
     }
+
     for (int k = 0; k < a.K; ++k) {
-        uint64_t best = key[0];
-        int at = 0;
+        uint32_t best = key[0];
 #pragma unroll
-        for (int j = 1; j < V; ++j)
-            if (key[j] > best) {
-                best = key[j];
-                at = j;
+        for (int j = 1; j < V; ++j) best = key[j] > best ? key[j] : best;
+        const uint32_t top = route_max<G>(best);
+        uint32_t from = top;
+        if constexpr (BIASED) {
+            if (top > 1) {
+                const float v = route_value(top);
+                from = route_key(v - route_margin<SIGMOID>(s_max, v));
             }
-        const uint64_t top = group_max<G>(best);
-        const int e = group_min<G>(best == top ? e0 + at : 0x7fffffff);
-        if (top != 0) {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (e0 + j == e) {
-                    key[j] = 0;
-                    picked[slot][k] = (float)s[j];
-                }
-        } else if (li == 0) {
-            picked[slot][k] = 0.f;
         }
-        if (li == 0 && t0 < a.T) a.idx[t * a.K + k] = top != 0 ? e : -1;
+        uint32_t cand = 0;  // this lane's experts that may be the largest
+#pragma unroll
+        for (int j = 0; j < V; ++j) cand |= (key[j] >= from ? 1u : 0u) << j;
+        if (top == 0) cand = 0;
+        int at = __ffs(cand) - 1;
+        unsigned long long holders = __ballot(cand != 0) & mine;
+        if constexpr (BIASED) {
+            const bool several = (cand & (cand - 1)) != 0 || (cand != 0 && (holders & (holders - 1)) != 0);
+            if (__any(several && top > 1)) {
+                const double total = SIGMOID ? 1.0 : route_sum64<LT, G>(a, t, li, m);
+                double c = -INFINITY;
+                for (uint32_t left = top > 1 ? cand : 0; left; left &= left - 1) {
+                    const int j = __ffs(left) - 1;
+                    const double w = route_score64<SIGMOID>(route_load<LT>(a.logits, t * a.ld + e0 + j), m, total) +
+                                     (double)a.bias[e0 + j];
+                    if (w > c) {
+                        c = w;
+                        at = j;
+                    }
+                }
+                double most = c;
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
+                const unsigned long long wide_holders = __ballot(cand != 0 && (top <= 1 || c == most)) & mine;
+                if (top > 1) holders = wide_holders;
+            }
+        }
+        const bool winner = cand != 0 && __ffsll(holders) - 1 == lane;
+        if (winner) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) key[j] = j == at ? 0 : key[j];
+            chosen[slot][k] = e0 + at;
+        }
+        if (top == 0 && li == 0) chosen[slot][k] = -1;
     }
-    __syncthreads();
-    float total = 0.f;
-    for (int k = 0; k < a.K; ++k) total += picked[slot][k];
-    const float f = a.renorm ? (total == 0.f ? 0.f : a.scale / total) : a.scale;
-    if (t0 < a.T)
-        for (int k = li; k < a.K; k += G) a.gate[t * a.K + k] = picked[slot][k] * f;
+    wave_lds_fence();
+
+    // the weights of the selected experts; kRouteMaxK / G slots per lane at most
+    constexpr int kOwn = (kRouteMaxK + G - 1) / G;
+    int e[kOwn];
+    float w[kOwn], xs[kOwn], part = 0.f, most = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+        const int k = li + q * G;
+        e[q] = k < a.K ? chosen[slot][k] : -1;
+        xs[q] = e[q] >= 0 ? route_load<LT>(a.logits, t * a.ld + e[q]) : -INFINITY;
+        most = fmaxf(most, xs[q]);
+    }
+    // renormalised softmax weights need no other expert: relative to the largest selected logit
+    if (!SIGMOID && a.renorm) most = route_fmax<G>(most);
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+        if (SIGMOID) w[q] = 1.0f / (1.0f + expf(-xs[q]));
+        else w[q] = a.renorm ? expf(xs[q] - most) : expf(xs[q] - m) / sum;
+        if (e[q] < 0) w[q] = 0.f;
+        part += w[q];
+    }
+    const float total = route_fsum<G>(part);
+#pragma unroll
+    for (int q = 0; q < kOwn; ++q) {
+        const int k = li + q * G;
+        if (k >= a.K || t0 >= a.T) continue;
+        a.idx[t * a.K + k] = e[q];
+        // (a token of no expert, or of scores that are all 0)
+        a.gate[t * a.K + k] = e[q] < 0 || (a.renorm && total == 0.f) ? 0.f : a.renorm ? a.scale * (w[q] / total) : a.scale * w[q];
+    }
 }
 
 // ---- backward -----------------------------------------------------------------------------------
-// With g'_k = s[idx_k] / S, S = sum_j s[idx_j]:
-//   d s[idx_k] = scale (dgate_k - sum_j g'_j dgate_j) / S   (renorm),   scale dgate_k   (otherwise)
+// With g'_k = s[idx_k] / sum_j s[idx_j]:
+//   d s[idx_k] = scale (dgate_k - sum_j g'_j dgate_j) / sum_j s[idx_j]   (renorm),   scale dgate_k   (otherwise)
 //   softmax: dx_e = s_e (ds_e - sum_j s_j ds_j);   sigmoid: dx_e = ds_e s_e (1 - s_e)
-// dgate_k is given, or <dout[t], y[pos(t, k)]> over the expert rows.  One wave per token.
+// Renormalised softmax weights are a softmax over the selected logits alone, dx_k = scale g'_k (dgate_k - sum g' dgate),
+// and sigmoid scores do not mix: only softmax weights that are not renormalised read the whole row.
+// dgate_k is given, or <dout[t], y[pos(t, k)]> over the expert rows.
+//
+// One wave per token; lane k < K holds slot k.  Bound by the expert rows: per chunk of 512 columns the loads of the
+// gradient row and of all K expert rows go out together.
 struct RouteBwdArgs {
     const void* logits;
     int64_t ld, T;
@@ -205,25 +410,91 @@ struct RouteBwdArgs {
     int32_t cols;  // columns E .. cols-1 of dlogits become zeros
 };
 
-template <typename LT, bool SIGMOID>
+__device__ __forceinline__ float route_dot8(const uint4& u, const uint4& v, float d) {
+    d = fmaf(bf16lo(u.x), bf16lo(v.x), d); d = fmaf(bf16hi(u.x), bf16hi(v.x), d);
+    d = fmaf(bf16lo(u.y), bf16lo(v.y), d); d = fmaf(bf16hi(u.y), bf16hi(v.y), d);
+    d = fmaf(bf16lo(u.z), bf16lo(v.z), d); d = fmaf(bf16hi(u.z), bf16hi(v.z), d);
+    d = fmaf(bf16lo(u.w), bf16lo(v.w), d); d = fmaf(bf16hi(u.w), bf16hi(v.w), d);
+    return d;
+}
+
+// KM: slots rounded up to a power of two
+template <typename LT, bool SIGMOID, int KM>
 __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a) {
     constexpr int V = kRouteMaxE / 64;
+    __shared__ float row[4][kRouteMaxE];
     const int lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= a.T) return;
-    float x[V];
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = j * 64 + lane;
-        x[j] = e < a.E ? route_load<LT>(a.logits, t * a.ld + e) : -INFINITY;
-        m = fmaxf(m, x[j]);
-    }
-    float s[V];
-    if constexpr (SIGMOID) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = 1.0f / (1.0f + expf(-x[j]));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    if (t >= a.T) return;  // (no work-group barrier below)
+    const bool slot = lane < a.K;
+    int e = slot ? a.idx[t * a.K + lane] : -1;
+    if (e >= a.E) e = -1;
+    const float xe = e >= 0 ? route_load<LT>(a.logits, t * a.ld + e) : -INFINITY;
+
+    float dg = 0.f;  // gradient of this lane's slot
+    if (a.dgate) {
+        if (e >= 0) dg = a.dgate[t * a.K + lane];
     } else {
+        const int pos = slot && e >= 0 ? a.pos[t * a.K + lane] : -1;
+        const uint4* rows[KM];
+        float acc[KM];
+        bool there[KM];
+#pragma unroll
+        for (int k = 0; k < KM; ++k) {
+            const int r = __builtin_amdgcn_readlane(pos, k);
+            there[k] = r >= 0;
+            rows[k] = reinterpret_cast<const uint4*>(a.y + (int64_t)(r >= 0 ? r : 0) * a.ld_y);
+            acc[k] = 0.f;
+        }
+        const uint4* op = reinterpret_cast<const uint4*>(a.dout + t * a.ld_dout);
+        for (int c = lane; c < a.C8; c += 64) {
+            const uint4 v = op[c];
+            uint4 u[KM];
+#pragma unroll
+            for (int k = 0; k < KM; ++k)
+                if (there[k]) u[k] = rows[k][c];
+#pragma unroll
+            for (int k = 0; k < KM; ++k)
+                if (there[k]) acc[k] = route_dot8(u[k], v, acc[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < KM; ++k) {
+            const float d = wave_sum(acc[k]);
+            if (lane == k && there[k]) dg = d;
+        }
+    }
+
+    float s[V], dx;
+    float dot = 0.f;
+    if (SIGMOID || a.renorm) {
+        float w;
+        if constexpr (SIGMOID) {
+            w = e >= 0 ? 1.0f / (1.0f + expf(-xe)) : 0.f;
+        } else {
+            const float most = wave_max(xe);
+            w = e >= 0 ? expf(xe - most) : 0.f;
+        }
+        float ds = a.scale * dg;
+        if (a.renorm) {
+            // differences against the first slot's gradient (the weights sum to one): a token with a single expert
+            // gets exactly no gradient
+            const float total = wave_sum(w), g = total == 0.f ? 0.f : w / total;
+            const float rel = dg - __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(dg)));
+            ds = a.scale * (rel - wave_sum(e >= 0 ? g * rel : 0.f));
+            dx = SIGMOID ? (total == 0.f ? 0.f : ds / total * w * (1.0f - w)) : ds * g;
+        } else {
+            dx = ds * w * (1.0f - w);
+        }
+        if (e < 0) dx = 0.f;
+    } else {
+        float x[V], m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = j * 64 + lane;
+            x[j] = c < a.E ? route_load<LT>(a.logits, t * a.ld + c) : -INFINITY;
+            m = fmaxf(m, x[j]);
+        }
         m = wave_max(m);
         float sum = 0.f;
 #pragma unroll
@@ -235,96 +506,45 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // no expert is there: no score, no gradient
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] *= inv;
+        const float ds = e >= 0 ? a.scale * dg : 0.f, w = e >= 0 ? expf(xe - m) * inv : 0.f;
+        dot = wave_sum(e >= 0 ? w * ds : 0.f);
+        dx = ds;
     }
-    // the slots of this token: gradient of the weight and the score, in every lane
-    float dg[kRouteMaxK], sk[kRouteMaxK];
-    float total = 0.f;
+    // slots of one expert add up (in slot order), then the row goes out
+    float mine = 0.f;
 #pragma unroll
-    for (int k = 0; k < kRouteMaxK; ++k) {
-        dg[k] = sk[k] = 0.f;
-        if (k >= a.K) break;
-        const int e = a.idx[t * a.K + k];
-        if (e < 0 || e >= a.E) continue;
-        if (a.dgate) {
-            dg[k] = a.dgate[t * a.K + k];
-        } else {
-            const int r = a.pos[t * a.K + k];
-            if (r >= 0) {
-                float d = 0.f;
-                const uint4* yp = reinterpret_cast<const uint4*>(a.y + (int64_t)r * a.ld_y);
-                const uint4* op = reinterpret_cast<const uint4*>(a.dout + t * a.ld_dout);
-                for (int c = lane; c < a.C8; c += 64) {
-                    const uint4 u = yp[c], v = op[c];
-                    d = fmaf(bf16lo(u.x), bf16lo(v.x), d); d = fmaf(bf16hi(u.x), bf16hi(v.x), d);
-                    d = fmaf(bf16lo(u.y), bf16lo(v.y), d); d = fmaf(bf16hi(u.y), bf16hi(v.y), d);
-                    d = fmaf(bf16lo(u.z), bf16lo(v.z), d); d = fmaf(bf16hi(u.z), bf16hi(v.z), d);
-                    d = fmaf(bf16lo(u.w), bf16lo(v.w), d); d = fmaf(bf16hi(u.w), bf16hi(v.w), d);
-                }
-                dg[k] = wave_sum(d);
-            }
-        }
-        float own = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j * 64 + lane == e) own = s[j];
-        sk[k] = __shfl(own, e & 63, 64);
-        total += sk[k];
+    for (int k = 0; k < KM; ++k) {
+        const int ek = __builtin_amdgcn_readlane(e, k);
+        const float dk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(dx), k));
+        if (ek == e) mine += dk;
     }
-    // With renorm the differences are taken against the first slot's gradient (the weights sum to one): a token
-    // with a single expert gets exactly no gradient.  Then sum_j s_j ds_j is zero, and softmax scores pass
-    // nothing on to the experts that were not selected.
-    float dot = 0.f;  // sum_j s_j ds_j over the selected experts
-    float along = 0.f;
-    if (a.renorm) {
-        const float ref = dg[0];
-#pragma unroll
-        for (int k = 0; k < kRouteMaxK; ++k) {
-            if (k >= a.K) break;
-            dg[k] -= ref;
-            along = fmaf(sk[k], dg[k], along);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < kRouteMaxK; ++k) {
-        if (k >= a.K) break;
-        if (a.renorm) {
-            dg[k] = total == 0.f ? 0.f : a.scale * (dg[k] - along / total) / total;
-        } else {
-            dg[k] *= a.scale;
-            dot = fmaf(sk[k], dg[k], dot);
-        }
-    }
-    float d[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) d[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < kRouteMaxK; ++k) {
-        if (k >= a.K) break;
-        const int e = a.idx[t * a.K + k];
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j * 64 + lane == e) d[j] += dg[k];
-    }
+    for (int c = lane; c < a.E; c += 64) row[wave][c] = 0.f;
+    wave_lds_fence();
+    if (e >= 0) row[wave][e] = mine;
+    wave_lds_fence();
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int e = j * 64 + lane;
-        if (e >= a.cols) continue;
-        float dx = 0.f;
-        if (e < a.E) dx = SIGMOID ? d[j] * s[j] * (1.0f - s[j]) : s[j] * (d[j] - dot);
-        if constexpr (sizeof(LT) == 2) static_cast<uint16_t*>(a.dlogits)[t * a.ld_dl + e] = f32_to_bf16(dx);
-        else static_cast<float*>(a.dlogits)[t * a.ld_dl + e] = dx;
+        const int c = j * 64 + lane;
+        if (c >= a.cols) break;
+        float v = c < a.E ? row[wave][c] : 0.f;
+        if (!SIGMOID && !a.renorm) v = c < a.E ? s[j] * (v - dot) : 0.f;
+        if constexpr (sizeof(LT) == 2) static_cast<uint16_t*>(a.dlogits)[t * a.ld_dl + c] = f32_to_bf16(v);
+        else static_cast<float*>(a.dlogits)[t * a.ld_dl + c] = v;
     }
 }
 
 // ---- permutation --------------------------------------------------------------------------------
-// A stable counting sort by expert.  A work-group takes kPermSlots consecutive slots, a wave a consecutive part
-// of them.  First launch: the counts of every work-group.  Second launch: every work-group adds up the counts
-// in front of it, ranks its slots in order and places them.  A wave finds the lanes that hold the same expert
-// from one ballot per bit of the expert index; the first of them does the counting for all.
+// A stable counting sort by expert.  A work-group takes kPermSlots consecutive slots, a wave a consecutive part of
+// them, 64 at a time: one ballot per bit of the expert index gives every lane the set of lanes that hold its
+// expert; its rank is the wave's count so far plus the members in front of it, and the first member counts for all.
+// Up to kPermSlots slots are one launch.  More are two: the counts of every work-group, then every work-group
+// adds up the counts of all and of those in front of it and places its slots.
+// 16 waves of 256 slots: twice as many work-groups of half the size double the counts that each one reads.
 constexpr int kPermMaxE = 1024;
-constexpr int kPermThreads = 256;
-constexpr int kPermSlots = 2048;
+constexpr int kPermThreads = 1024;
 constexpr int kPermWaves = kPermThreads / 64;
+constexpr int kPermRounds = 4;
+constexpr int kPermSlots = kPermThreads * kPermRounds;
 
 __device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
     unsigned long long m = __ballot(e >= 0);
@@ -335,27 +555,27 @@ __device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
     return m;
 }
 
-__device__ __forceinline__ int perm_expert(const int32_t* ids, int64_t i, int64_t n, int E) {
-    const int e = i < n ? ids[i] : -1;
-    return e >= 0 && e < E ? e : -1;
-}
-
-// Orders a wave's LDS accesses with those of its other lanes.
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// Counts of this work-group's waves into cnt[wave][E].
-__device__ __forceinline__ void perm_count(int (*cnt)[kPermMaxE], const int32_t* ids, int64_t n, int E, int bits) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < kPermWaves * kPermMaxE; i += kPermThreads) (&cnt[0][0])[i] = 0;
-    __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * kPermSlots + wave * (kPermSlots / kPermWaves);
-    for (int q = 0; q < kPermSlots / kPermWaves; q += 64) {
-        const int e = perm_expert(ids, first + q + lane, n, E);
-        const unsigned long long m = same_expert(e, bits);
-        if (e >= 0 && __ffsll(m) - 1 == lane) cnt[wave][e] += __popcll(m);
+// Ranks this work-group's slots inside their wave: e[q] the expert of the lane's q-th slot (-1: none), r[q] its rank;
+// cnt[wave][E] the wave's counts.
+__device__ __forceinline__ void perm_rank(int (*cnt)[kPermMaxE], const int32_t* ids, int64_t n, int E, int bits,
+                                          int (&e)[kPermRounds], int (&r)[kPermRounds]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = (int64_t)blockIdx.x * kPermSlots + wave * (64 * kPermRounds) + lane;
+#pragma unroll
+    for (int q = 0; q < kPermRounds; ++q) {
+        e[q] = first + q * 64 < n ? ids[first + q * 64] : -1;
+        if (e[q] >= E) e[q] = -1;
+    }
+    for (int i = lane; i < E; i += 64) cnt[wave][i] = 0;
+    wave_lds_fence();
+#pragma unroll
+    for (int q = 0; q < kPermRounds; ++q) {
+        const unsigned long long m = same_expert(e[q], bits);
+        r[q] = 0;
+        if (e[q] >= 0) r[q] = cnt[wave][e[q]] + __popcll(m & ((1ull << lane) - 1ull));
+        // every lane has read before the first lane of a set writes, and that is written before the next round
+        wave_lds_fence();
+        if (e[q] >= 0 && __ffsll(m) - 1 == lane) cnt[wave][e[q]] = r[q] + __popcll(m);
         wave_lds_fence();
     }
     __syncthreads();
@@ -364,11 +584,13 @@ __device__ __forceinline__ void perm_count(int (*cnt)[kPermMaxE], const int32_t*
 __global__ __launch_bounds__(kPermThreads) void moe_permute_count_kernel(const int32_t* __restrict__ ids, int64_t n,
                                                                          int E, int bits, int32_t* __restrict__ ws) {
     __shared__ int cnt[kPermWaves][kPermMaxE];
-    perm_count(cnt, ids, n, E, bits);
-    for (int e = threadIdx.x; e < E; e += kPermThreads) {
+    int e[kPermRounds], r[kPermRounds];
+    perm_rank(cnt, ids, n, E, bits, e, r);
+    if ((int)threadIdx.x < E) {
         int s = 0;
-        for (int w = 0; w < kPermWaves; ++w) s += cnt[w][e];
-        ws[(int64_t)blockIdx.x * E + e] = s;
+#pragma unroll
+        for (int w = 0; w < kPermWaves; ++w) s += cnt[w][threadIdx.x];
+        ws[(int64_t)blockIdx.x * E + threadIdx.x] = s;
     }
 }
 
@@ -378,77 +600,85 @@ __global__ __launch_bounds__(kPermThreads) void moe_permute_place_kernel(const i
                                                                          int32_t* __restrict__ row_src,
                                                                          int32_t* __restrict__ pos) {
     __shared__ int cnt[kPermWaves][kPermMaxE];
-    __shared__ int sum[kPermThreads];
+    __shared__ int wave_total[kPermWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    perm_count(cnt, ids, n, E, bits);
-    // per expert (4 consecutive ones per thread): its total, and what lies in front of this work-group
-    constexpr int V = kPermMaxE / kPermThreads;
-    int total[V], before[V], mine = 0;
-    for (int j = 0; j < V; ++j) {
-        const int e = tid * V + j;
-        total[j] = before[j] = 0;
-        if (e < E)
+    int e[kPermRounds], r[kPermRounds];
+    perm_rank(cnt, ids, n, E, bits, e, r);
+    // expert tid: its total over all work-groups, and what lies in front of this one
+    int total = 0, before = 0;
+    if (tid < E) {
+        if (gridDim.x == 1) {
+#pragma unroll
+            for (int w = 0; w < kPermWaves; ++w) total += cnt[w][tid];
+        } else {
+#pragma unroll 16
             for (unsigned b = 0; b < gridDim.x; ++b) {
-                const int v = ws[(int64_t)b * E + e];
-                total[j] += v;
-                if (b < blockIdx.x) before[j] += v;
-            }
-        mine += total[j];
-    }
-    sum[tid] = mine;
-    __syncthreads();
-    for (int o = 1; o < kPermThreads; o <<= 1) {
-        const int add = tid >= o ? sum[tid - o] : 0;
-        __syncthreads();
-        sum[tid] += add;
-        __syncthreads();
-    }
-    int begin = sum[tid] - mine;
-    for (int j = 0; j < V; ++j) {
-        const int e = tid * V + j;
-        if (e < E) {
-            if (blockIdx.x == 0) seg_start[e] = begin;
-            int at = begin + before[j];  // the waves of this work-group, one after the other
-            for (int w = 0; w < kPermWaves; ++w) {
-                const int v = cnt[w][e];
-                cnt[w][e] = at;
-                at += v;
+                const int v = ws[(int64_t)b * E + tid];
+                total += v;
+                before += b < blockIdx.x ? v : 0;
             }
         }
-        begin += total[j];
     }
-    if (blockIdx.x == 0 && tid == kPermThreads - 1) seg_start[E] = sum[tid];
+    int upto = total;  // running sum over the experts: inside the wave, then over the waves
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int add = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += add;
+    }
+    if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * kPermSlots + wave * (kPermSlots / kPermWaves);
-    for (int q = 0; q < kPermSlots / kPermWaves; q += 64) {
-        const int64_t i = first + q + lane;
-        const int e = perm_expert(ids, i, n, E);
-        const unsigned long long m = same_expert(e, bits);
-        int r = -1;
-        if (e >= 0) r = cnt[wave][e] + __popcll(m & ((1ull << lane) - 1ull));
-        // every lane has read before the first lane of a set writes, and that is written before the next round
-        wave_lds_fence();
-        if (e >= 0 && __ffsll(m) - 1 == lane) cnt[wave][e] = r + __popcll(m);
-        wave_lds_fence();
-        if (i < n) {
-            pos[i] = r;
-            if (r >= 0) row_src[r] = (int)i;
+    for (int w = 0; w < wave; ++w) upto += wave_total[w];
+    if (tid < E) {
+        const int begin = upto - total;
+        if (blockIdx.x == 0) {
+            seg_start[tid] = begin;
+            if (tid == E - 1) seg_start[E] = upto;
         }
+        int at = begin + before;  // the waves of this work-group, one after the other
+#pragma unroll
+        for (int w = 0; w < kPermWaves; ++w) {
+            const int v = cnt[w][tid];
+            cnt[w][tid] = at;
+            at += v;
+        }
+    }
+    __syncthreads();
+    const int64_t first = (int64_t)blockIdx.x * kPermSlots + wave * (64 * kPermRounds) + lane;
+#pragma unroll
+    for (int q = 0; q < kPermRounds; ++q) {
+        const int64_t i = first + q * 64;
+        if (i >= n) continue;
+        const int at = e[q] >= 0 ? cnt[wave][e[q]] + r[q] : -1;
+        pos[i] = at;
+        if (at >= 0) row_src[at] = (int)i;
     }
 }
 
 static int64_t perm_groups(int64_t n) { return n > 0 ? (n + kPermSlots - 1) / kPermSlots : 1; }
 
-template <typename LT, bool SIGMOID, bool TOP2>
+template <typename LT, bool SIGMOID, bool BIASED>
 static int route_launch(const RouteArgs& a, hipStream_t st) {
     auto go = [&](auto kernel, int tokens) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((a.T + tokens - 1) / tokens)), dim3(256), 0, st, a);
         return check_launch("moe_route_kernel");
     };
-    if (a.E <= 16) return go(moe_route_kernel<LT, 8, 2, SIGMOID, TOP2>, 32);
-    if (a.E <= 64) return go(moe_route_kernel<LT, 16, 4, SIGMOID, TOP2>, 16);
-    if (a.E <= 256) return go(moe_route_kernel<LT, 32, 8, SIGMOID, TOP2>, 8);
-    return go(moe_route_kernel<LT, 64, 8, SIGMOID, TOP2>, 4);
+    if (a.E <= 16) return go(moe_route_kernel<LT, 8, 2, SIGMOID, BIASED>, 32);
+    if (a.E <= 64) return go(moe_route_kernel<LT, 8, 8, SIGMOID, BIASED>, 32);
+    if (a.E <= 128) return go(moe_route_kernel<LT, 16, 8, SIGMOID, BIASED>, 16);
+    if (a.E <= 256) return go(moe_route_kernel<LT, 16, 16, SIGMOID, BIASED>, 16);
+    return go(moe_route_kernel<LT, 32, 16, SIGMOID, BIASED>, 8);
+}
+
+template <typename LT, bool SIGMOID>
+static int route_bwd_launch(const RouteBwdArgs& a, hipStream_t st) {
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.T + 3) / 4)), dim3(256), 0, st, a);
+        return check_launch("moe_route_bwd_kernel");
+    };
+    if (a.K <= 2) return go(moe_route_bwd_kernel<LT, SIGMOID, 2>);
+    if (a.K <= 4) return go(moe_route_bwd_kernel<LT, SIGMOID, 4>);
+    if (a.K <= 8) return go(moe_route_bwd_kernel<LT, SIGMOID, 8>);
+    return go(moe_route_bwd_kernel<LT, SIGMOID, 16>);
 }
 
 static int route_check(const char* who, const pp_moe_route_desc* d) {
@@ -485,13 +715,16 @@ extern "C" int pp_moe_route(const pp_moe_route_desc* d, pp_stream stream) {
     a.E = d->E; a.K = d->topk; a.n_group = ng; a.topk_group = kg;
     a.renorm = d->renorm; a.scale = d->scale; a.idx = d->topk_idx; a.gate = d->gate;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool sig = d->scoring == PP_MOE_SIGMOID, top2 = d->group_score == PP_MOE_GROUP_TOP2;
+    const int64_t size = d->dtype == PP_BF16 ? 2 : 4;
+    a.group_top2 = d->group_score == PP_MOE_GROUP_TOP2;
+    a.vec = aligned(d->logits, 16) && d->ld * size % 16 == 0;
+    const bool sig = d->scoring == PP_MOE_SIGMOID, biased = d->bias != nullptr;
     if (d->dtype == PP_BF16) {
-        if (sig) return top2 ? route_launch<uint16_t, true, true>(a, st) : route_launch<uint16_t, true, false>(a, st);
-        return top2 ? route_launch<uint16_t, false, true>(a, st) : route_launch<uint16_t, false, false>(a, st);
+        if (sig) return biased ? route_launch<uint16_t, true, true>(a, st) : route_launch<uint16_t, true, false>(a, st);
+        return biased ? route_launch<uint16_t, false, true>(a, st) : route_launch<uint16_t, false, false>(a, st);
     }
-    if (sig) return top2 ? route_launch<float, true, true>(a, st) : route_launch<float, true, false>(a, st);
-    return top2 ? route_launch<float, false, true>(a, st) : route_launch<float, false, false>(a, st);
+    if (sig) return biased ? route_launch<float, true, true>(a, st) : route_launch<float, true, false>(a, st);
+    return biased ? route_launch<float, false, true>(a, st) : route_launch<float, false, false>(a, st);
 }
 
 extern "C" int pp_moe_route_bwd(const pp_moe_route_desc* d, pp_stream stream) {
@@ -515,13 +748,9 @@ extern "C" int pp_moe_route_bwd(const pp_moe_route_desc* d, pp_stream stream) {
     a.pos = d->pos; a.C8 = (int32_t)(d->C / 8);
     a.dlogits = d->dlogits; a.ld_dl = d->ld_dl; a.cols = d->cols_dl;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.T + 3) / 4)), dim3(256), 0, st, a);
-        return check_launch("moe_route_bwd_kernel");
-    };
     const bool sig = d->scoring == PP_MOE_SIGMOID;
-    if (d->dtype == PP_BF16) return sig ? go(moe_route_bwd_kernel<uint16_t, true>) : go(moe_route_bwd_kernel<uint16_t, false>);
-    return sig ? go(moe_route_bwd_kernel<float, true>) : go(moe_route_bwd_kernel<float, false>);
+    if (d->dtype == PP_BF16) return sig ? route_bwd_launch<uint16_t, true>(a, st) : route_bwd_launch<uint16_t, false>(a, st);
+    return sig ? route_bwd_launch<float, true>(a, st) : route_bwd_launch<float, false>(a, st);
 }
 
 extern "C" int64_t pp_moe_permute_workspace_ints(int64_t n_slots, int E) {
@@ -543,9 +772,11 @@ extern "C" int pp_moe_permute_ws(const int32_t* expert_of_slot, int64_t n_slots,
     while ((1 << bits) < E) ++bits;
     const dim3 grid((unsigned)perm_groups(n_slots));
     hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(moe_permute_count_kernel, grid, dim3(kPermThreads), 0, st, expert_of_slot, n_slots, E, bits, workspace);
-    int rc = check_launch("moe_permute_count_kernel");
-    if (rc) return rc;
+    if (grid.x > 1) {
+        hipLaunchKernelGGL(moe_permute_count_kernel, grid, dim3(kPermThreads), 0, st, expert_of_slot, n_slots, E, bits, workspace);
+        const int rc = check_launch("moe_permute_count_kernel");
+        if (rc) return rc;
+    }
     hipLaunchKernelGGL(moe_permute_place_kernel, grid, dim3(kPermThreads), 0, st, expert_of_slot, n_slots, E, bits, workspace,
                        seg_start, row_src, pos);
     return check_launch("moe_permute_place_kernel");
