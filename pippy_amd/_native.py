@@ -236,14 +236,18 @@ def _need(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _require_here(*tensors: Optional[torch.Tensor]) -> None:
-    """Device tensors of the current device, where the launch goes."""
-    require_cuda(*tensors)
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != here:
-            raise RuntimeError(f"tensor on {t.device}, but the current device is cuda:{here}: make the tensors' "
-                               "device the current one around the call (torch.cuda.device)")
+def _stream_for(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The current stream, for tensors that all live on the current device (where a launch goes)."""
+    dev = first.get_device()        # -1: host memory
+    ok = dev >= 0 and dev == torch._C._cuda_getDevice()
+    for t in others:
+        ok = ok and (t is None or t.get_device() == dev)
+    if not ok:
+        require_cuda(first, *others)
+        raise RuntimeError(f"tensors on {sorted({str(t.device) for t in (first, *others) if t is not None})}, the current "
+                           f"device is cuda:{torch.cuda.current_device()}: make the tensors' device the current one "
+                           "around the call (torch.cuda.device)")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 # ---- microbatch copies ----------------------------------------------------------------------
@@ -529,21 +533,23 @@ def moe_gate_bwd(dout, y, pos, topk_idx, gate, E: int, dlogits) -> None:
                                 dlogits.stride(0), T, Cc, current_stream()), "pp_moe_gate_bwd")
 
 
-def _moe_route_desc(who, logits, topk_idx, scoring, renorm, scale, E) -> MoeRouteDesc:
-    _need(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1) and topk_idx.dim() == 2,
-          f"{who}: logits [tokens, experts] with contiguous rows and topk_idx [tokens, k]")
+def _moe_slots(who, topk_idx, t, T, name, dtype):
+    _need(t.dtype == dtype and t.is_contiguous() and t.shape == topk_idx.shape,
+          f"{who}: {name} must be contiguous {dtype} of topk_idx's shape")
+
+
+def _moe_logits(who, logits, topk_idx, scoring, E):
+    """(rows, row stride, experts) of the logits."""
+    _need(logits.dim() == 2 and topk_idx.dim() == 2, f"{who}: logits [tokens, experts] and topk_idx [tokens, k]")
     T, cols = logits.shape
+    ld, step = logits.stride()
     E = cols if E is None else E
+    _need(step == 1 or cols == 1, f"{who}: the rows of logits must be contiguous")
     _need(topk_idx.shape[0] == T and topk_idx.dtype == torch.int32 and topk_idx.is_contiguous(),
           f"{who}: topk_idx must be contiguous int32 with a row per token")
     _need(2 <= E <= cols, f"{who}: {E} experts in {cols} columns")
     _need(scoring in MOE_SCORING, f"{who}: scoring {scoring!r}; known: {sorted(MOE_SCORING)}")
-    d = MoeRouteDesc()
-    d.logits, d.ld, d.T = logits.data_ptr(), max(logits.stride(0), cols), T
-    d.topk_idx = topk_idx.data_ptr()
-    d.dtype, d.E, d.topk = _pp_dtype(logits), E, topk_idx.shape[1]
-    d.scoring, d.renorm, d.scale = MOE_SCORING[scoring], int(renorm), scale
-    return d
+    return T, ld if T > 1 else cols, E
 
 
 def moe_route(logits, topk_idx, gate, *, bias=None, scoring: str = "softmax", n_group: int = 1, topk_group: int = 1,
@@ -551,16 +557,16 @@ def moe_route(logits, topk_idx, gate, *, bias=None, scoring: str = "softmax", n_
     """The ``k`` experts of every token and their weights (see ``pp_moe_route``): ``logits`` [T, experts] bf16 or
     fp32, ``topk_idx`` int32 [T, k] and ``gate`` fp32 [T, k] are written.  ``E``: the number of experts when
     ``logits`` carries padding columns after them; ``bias`` fp32 [E] enters the selection only."""
-    _require_here(logits, topk_idx, gate, bias)
-    d = _moe_route_desc("moe_route", logits, topk_idx, scoring, renorm, scale, E)
-    _need(gate.shape == topk_idx.shape and gate.dtype == torch.float32 and gate.is_contiguous(),
-          "moe_route: gate must be contiguous fp32 of topk_idx's shape")
-    _need(bias is None or (bias.shape == (d.E,) and bias.dtype == torch.float32 and bias.is_contiguous()),
-          f"moe_route: bias must be contiguous fp32 [{d.E}]")
+    stream = _stream_for(logits, topk_idx, gate, bias)
+    T, ld, E = _moe_logits("moe_route", logits, topk_idx, scoring, E)
+    _moe_slots("moe_route", topk_idx, gate, T, "gate", torch.float32)
+    _need(bias is None or (bias.shape == (E,) and bias.dtype == torch.float32 and bias.is_contiguous()),
+          f"moe_route: bias must be contiguous fp32 [{E}]")
     _need(group_score in MOE_GROUP_SCORE, f"moe_route: group_score {group_score!r}; known: {sorted(MOE_GROUP_SCORE)}")
-    d.gate, d.bias = gate.data_ptr(), ptr(bias)
-    d.n_group, d.topk_group, d.group_score = n_group, topk_group, MOE_GROUP_SCORE[group_score]
-    check(lib().pp_moe_route(C.byref(d), current_stream()), "pp_moe_route")
+    d = MoeRouteDesc(logits.data_ptr(), ld, T, ptr(bias), topk_idx.data_ptr(), gate.data_ptr(), _pp_dtype(logits), E,
+                     topk_idx.shape[1], MOE_SCORING[scoring], n_group, topk_group, MOE_GROUP_SCORE[group_score], renorm,
+                     scale)
+    check(lib().pp_moe_route(C.byref(d), stream), "pp_moe_route")
 
 
 def moe_route_bwd(logits, topk_idx, dlogits, *, dgate=None, dout=None, y=None, pos=None, scoring: str = "softmax",
@@ -568,29 +574,30 @@ def moe_route_bwd(logits, topk_idx, dlogits, *, dgate=None, dout=None, y=None, p
     """Gradient of the router logits (see ``pp_moe_route_bwd``) from the gradient of the weights, ``dgate`` fp32
     [T, k], or from the output gradient ``dout`` [T, C], the expert rows ``y`` [rows, C] and their positions ``pos``
     [T * k].  ``dlogits`` [T, columns >= E] has the type of ``logits``; columns past the experts become zeros."""
-    _require_here(logits, topk_idx, dlogits, dgate, dout, y, pos)
-    d = _moe_route_desc("moe_route_bwd", logits, topk_idx, scoring, renorm, scale, E)
-    _need(dlogits.dim() == 2 and dlogits.shape[0] == d.T and dlogits.shape[1] >= d.E and
-          dlogits.dtype == logits.dtype and dlogits.stride(1) == 1,
-          "moe_route_bwd: dlogits [tokens, at least the experts] of the type of logits")
-    d.dlogits, d.ld_dl, d.cols_dl = dlogits.data_ptr(), max(dlogits.stride(0), dlogits.shape[1]), dlogits.shape[1]
+    stream = _stream_for(logits, topk_idx, dlogits, dgate, dout, y, pos)
+    T, ld, E = _moe_logits("moe_route_bwd", logits, topk_idx, scoring, E)
+    _need(dlogits.dim() == 2 and dlogits.shape[0] == T and dlogits.shape[1] >= E and dlogits.dtype == logits.dtype and
+          dlogits.stride(1) == 1, "moe_route_bwd: dlogits [tokens, at least the experts] of the type of logits")
+    width = ld_dout = ld_y = 0
     if dgate is not None:
-        _need(dgate.shape == topk_idx.shape and dgate.dtype == torch.float32 and dgate.is_contiguous(),
-              "moe_route_bwd: dgate must be contiguous fp32 of topk_idx's shape")
-        d.dgate = dgate.data_ptr()
+        _moe_slots("moe_route_bwd", topk_idx, dgate, T, "dgate", torch.float32)
+        dout = y = pos = None
     else:
         _need(dout is not None and y is not None and pos is not None,
               "moe_route_bwd: needs dgate, or dout, y and pos")
-        _need(dout.dim() == 2 and y.dim() == 2 and dout.shape[0] == d.T and dout.shape[1] == y.shape[1] and
+        _need(dout.dim() == 2 and y.dim() == 2 and dout.shape[0] == T and dout.shape[1] == y.shape[1] and
               dout.dtype == y.dtype == torch.bfloat16 and dout.stride(1) == 1 and y.stride(1) == 1,
               "moe_route_bwd: dout [tokens, C] and y [rows, C] must be bf16 with contiguous rows")
         _need(pos.numel() == topk_idx.numel() and pos.dtype == torch.int32 and pos.is_contiguous(),
               "moe_route_bwd: pos must be contiguous int32 with an entry per slot")
-        d.dout, d.y, d.pos = dout.data_ptr(), y.data_ptr(), pos.data_ptr()
-        d.C = dout.shape[1]
-        d.ld_dout = dout.stride(0) if d.T > 1 else d.C
-        d.ld_y = y.stride(0) if y.shape[0] > 1 else d.C
-    check(lib().pp_moe_route_bwd(C.byref(d), current_stream()), "pp_moe_route_bwd")
+        width = dout.shape[1]
+        ld_dout = dout.stride(0) if T > 1 else width
+        ld_y = y.stride(0) if y.shape[0] > 1 else width
+    d = MoeRouteDesc(logits.data_ptr(), ld, T, None, topk_idx.data_ptr(), None, _pp_dtype(logits), E, topk_idx.shape[1],
+                     MOE_SCORING[scoring], 1, 1, 0, renorm, scale, dlogits.shape[1], ptr(dgate), ptr(dout), ptr(y),
+                     ptr(pos), ld_dout, ld_y, width, dlogits.data_ptr(),
+                     dlogits.stride(0) if T > 1 else dlogits.shape[1])
+    check(lib().pp_moe_route_bwd(C.byref(d), stream), "pp_moe_route_bwd")
 
 
 def moe_permute_workspace(n_slots: int, E: int) -> int:
@@ -602,28 +609,31 @@ def moe_permute_workspace(n_slots: int, E: int) -> int:
 
 def moe_permute_ws(expert_of_slot, E: int, seg_start, row_src, pos, workspace) -> None:
     """``moe_permute`` for up to 1024 experts and many slots (``workspace``: int32, ``moe_permute_workspace``)."""
-    _require_here(expert_of_slot, seg_start, row_src, pos, workspace)
+    stream = _stream_for(expert_of_slot, seg_start, row_src, pos, workspace)
     n = expert_of_slot.numel()
     for t in (expert_of_slot, seg_start, row_src, pos, workspace):
         _need(t.dtype == torch.int32 and t.is_contiguous(), "moe_permute_ws: tensors must be contiguous int32")
     _need(seg_start.numel() == E + 1 and row_src.numel() == n and pos.numel() == n,
           "moe_permute_ws: seg_start [E + 1], row_src and pos an entry per slot")
     check(lib().pp_moe_permute_ws(expert_of_slot.data_ptr(), n, E, seg_start.data_ptr(), row_src.data_ptr(),
-                                  pos.data_ptr(), workspace.data_ptr(), workspace.numel(), current_stream()),
+                                  pos.data_ptr(), workspace.data_ptr(), workspace.numel(), stream),
           "pp_moe_permute_ws")
 
 
 # ---- dropout ------------------------------------------------------------------------------------
-def _dropout_rows(*tensors):
-    """(rows, C, leading dimensions): one flat row when all are contiguous, else rows of the last dimension."""
-    x = tensors[0]
-    for t in tensors:
-        _need(t is None or (t.shape == x.shape and t.dtype == x.dtype), "dropout: tensors of one shape and type")
-    if all(t is None or t.is_contiguous() for t in tensors):
-        return 1, x.numel(), [x.numel()] * len(tensors)
-    _need(x.dim() == 2 and all(t is None or t.stride(1) == 1 for t in tensors),
+def _dropout_rows(x, y, resid):
+    """(rows, C, leading dimensions of x, resid, y): one flat row when all are contiguous, else rows of the last
+    dimension."""
+    shape, dtype = x.shape, x.dtype
+    _need(y.shape == shape and y.dtype == dtype and (resid is None or (resid.shape == shape and resid.dtype == dtype)),
+          "dropout: tensors of one shape and type")
+    if x.is_contiguous() and y.is_contiguous() and (resid is None or resid.is_contiguous()):
+        n = x.numel()
+        return 1, n, n, n, n
+    _need(len(shape) == 2 and all(t is None or t.stride(1) == 1 for t in (x, y, resid)),
           "dropout: contiguous tensors, or two-dimensional ones with contiguous rows")
-    return x.shape[0], x.shape[1], [0 if t is None else max(t.stride(0), x.shape[1]) for t in tensors]
+    ld = [0 if t is None else max(t.stride(0), shape[1]) for t in (x, resid, y)]
+    return (shape[0], shape[1], *ld)
 
 
 def _dropout_rng(rng) -> int:
@@ -634,24 +644,24 @@ def _dropout_rng(rng) -> int:
 def dropout_add(x, y, rng, p: float, *, resid=None, site: int = 0) -> None:
     """y = resid + mask * x / (1 - p) (see ``pp_dropout_add``).  ``rng``: int64 {seed, offset} on the device; a
     site and offset of its own for every mask that must differ."""
-    _require_here(x, y, rng, resid)
-    rows, Cc, (ld_x, ld_r, ld_y) = _dropout_rows(x, resid, y)
-    check(lib().pp_dropout_add(x.data_ptr(), ld_x, ptr(resid), ld_r, y.data_ptr(), ld_y, rows, Cc, _pp_dtype(x), p,
-                               _dropout_rng(rng), site, current_stream()), "pp_dropout_add")
+    stream = _stream_for(x, y, rng, resid)
+    rows, width, ld_x, ld_r, ld_y = _dropout_rows(x, y, resid)
+    check(lib().pp_dropout_add(x.data_ptr(), ld_x, ptr(resid), ld_r, y.data_ptr(), ld_y, rows, width, _pp_dtype(x), p,
+                               _dropout_rng(rng), site, stream), "pp_dropout_add")
 
 
 def dropout_bwd(dy, dx, rng, p: float, *, site: int = 0) -> None:
     """dx = mask * dy / (1 - p) under the mask of ``dropout_add`` with the same ``rng``, ``p`` and ``site``."""
-    _require_here(dy, dx, rng)
-    rows, Cc, (ld_dy, ld_dx) = _dropout_rows(dy, dx)
-    check(lib().pp_dropout_bwd(dy.data_ptr(), ld_dy, dx.data_ptr(), ld_dx, rows, Cc, _pp_dtype(dy), p,
-                               _dropout_rng(rng), site, current_stream()), "pp_dropout_bwd")
+    stream = _stream_for(dy, dx, rng)
+    rows, width, ld_dy, _, ld_dx = _dropout_rows(dy, dx, None)
+    check(lib().pp_dropout_bwd(dy.data_ptr(), ld_dy, dx.data_ptr(), ld_dx, rows, width, _pp_dtype(dy), p,
+                               _dropout_rng(rng), site, stream), "pp_dropout_bwd")
 
 
 def rng_advance(rng, step: int = 1) -> None:
     """Adds ``step`` to the offset of ``rng`` on the stream (inside a captured graph: on every replay)."""
-    _require_here(rng)
-    check(lib().pp_rng_advance(_dropout_rng(rng), step, current_stream()), "pp_rng_advance")
+    stream = _stream_for(rng)
+    check(lib().pp_rng_advance(_dropout_rng(rng), step, stream), "pp_rng_advance")
 
 
 def fill_bytes(t: torch.Tensor, value: int = 0) -> None:
@@ -913,6 +923,8 @@ def attn_bwd(qkv, o, lse, d_o, dqkv, delta, H, causal, scale=None, n_kv_heads=No
 class PackedPlan:
     """Which blocks of rows a packed batch has (see ``pp_attn_packed_plan``); made by ``attn_packed_plan``."""
 
+    __slots__ = ("ints", "n_seq", "rows")
+
     def __init__(self, ints: torch.Tensor, n_seq: int, rows: int):
         self.ints, self.n_seq, self.rows = ints, n_seq, rows
 
@@ -921,7 +933,7 @@ def attn_packed_plan(cu_seqlens: torch.Tensor, rows: int, out: Optional[PackedPl
     """The plan of a batch of ``rows`` rows whose sequence b lies in rows ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1``
     (int32 on the device).  One plan serves every layer and both directions of the batch.  ``out``: a plan for as
     many sequences and rows to write into (a captured graph rebuilds it in place on every replay)."""
-    _require_here(cu_seqlens)
+    stream = _stream_for(cu_seqlens, None if out is None else out.ints)
     _need(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and
           cu_seqlens.is_contiguous(), "attn_packed_plan: cu_seqlens must be contiguous int32 [sequences + 1]")
     n_seq = cu_seqlens.numel() - 1
@@ -930,55 +942,61 @@ def attn_packed_plan(cu_seqlens: torch.Tensor, rows: int, out: Optional[PackedPl
         _need(n >= 0, f"attn_packed_plan: {rows} rows are out of range")
         out = PackedPlan(torch.empty(n, dtype=torch.int32, device=cu_seqlens.device), n_seq, rows)
     _need(out.n_seq == n_seq and out.rows == rows, "attn_packed_plan: `out` is a plan of other sizes")
-    _require_here(out.ints)
-    check(lib().pp_attn_packed_plan(cu_seqlens.data_ptr(), n_seq, rows, out.ints.data_ptr(), current_stream()),
+    check(lib().pp_attn_packed_plan(cu_seqlens.data_ptr(), n_seq, rows, out.ints.data_ptr(), stream),
           "pp_attn_packed_plan")
     return out
 
 
-def attn_packed_desc(q, k, v, o, lse, plan: PackedPlan, causal: bool = True, scale: Optional[float] = None,
-                     d_o=None, dq=None, dk=None, dv=None, delta=None) -> AttnPackedDesc:
-    _require_here(q, k, v, o, lse, plan.ints, d_o, dq, dk, dv, delta)
+def _packed_rows(name, t, shape):
+    """(address, row stride) of a bf16 [rows, heads, D] tensor whose heads lie one after the other in a row."""
+    rows, heads, D = shape
+    if t.shape != shape or t.dtype != torch.bfloat16:
+        raise ValueError(f"packed attention: {name} must be bf16 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    stride, between, step = t.stride()
+    if step != 1 or (between != D and heads != 1):
+        raise ValueError(f"packed attention: the heads of a row of {name} must lie one after the other")
+    return t.data_ptr(), stride if rows > 1 else heads * D
+
+
+def _packed_stat(name, t, H, T):
+    _need(t.shape == (H, T) and t.dtype == torch.float32 and t.is_contiguous(),
+          f"packed attention: {name} must be contiguous fp32 {[H, T]}")
+    return t.data_ptr()
+
+
+def _packed_shapes(q, k, plan):
     _need(q.dim() == 3 and k.dim() == 3, "packed attention: q [rows, heads, D], k and v [rows, kv_heads, D]")
     T, H, D = q.shape
     Hkv = k.shape[1]
     _need(plan.rows == T, f"packed attention: a plan of {plan.rows} rows for tensors of {T}")
-    d = AttnPackedDesc()
-    for name, t, heads, stride in (("q", q, H, "stride_q"), ("k", k, Hkv, "stride_k"), ("v", v, Hkv, "stride_v"),
-                                   ("o", o, H, "stride_o"), ("d_o", d_o, H, "stride_do"), ("dq", dq, H, "stride_dq"),
-                                   ("dk", dk, Hkv, "stride_dk"), ("dv", dv, Hkv, "stride_dv")):
-        if t is None:
-            continue
-        _need(t.shape == (T, heads, D) and t.dtype == torch.bfloat16,
-              f"packed attention: {name} must be bf16 {[T, heads, D]}, got {t.dtype} {list(t.shape)}")
-        _need(t.stride(2) == 1 and (heads == 1 or t.stride(1) == D),
-              f"packed attention: the heads of a row of {name} must lie one after the other")
-        setattr(d, name, t.data_ptr())
-        setattr(d, stride, t.stride(0) if T > 1 else max(heads * D, 8))
-    for name, t in (("lse", lse), ("delta", delta)):
-        if t is None:
-            continue
-        _need(t.shape == (H, T) and t.dtype == torch.float32 and t.is_contiguous(),
-              f"packed attention: {name} must be contiguous fp32 {[H, T]}")
-        setattr(d, name, t.data_ptr())
-    d.plan, d.n_seq = plan.ints.data_ptr(), plan.n_seq
-    d.T, d.H, d.Hkv, d.D = T, H, Hkv, D
-    d.scale, d.causal = D ** -0.5 if scale is None else scale, int(causal)
-    return d
+    return T, H, Hkv, D, (T, H, D), (T, Hkv, D)
 
 
 def attn_packed_fwd(q, k, v, o, lse, plan: PackedPlan, *, causal: bool = True, scale: Optional[float] = None) -> None:
     """Attention over packed sequences (see ``pp_attn_packed_fwd``): ``o`` [rows, heads, D] and ``lse`` [heads, rows]
     are written for the rows of the sequences; other rows stay as they are."""
-    d = attn_packed_desc(q, k, v, o, lse, plan, causal, scale)
-    check(lib().pp_attn_packed_fwd(C.byref(d), current_stream()), "pp_attn_packed_fwd")
+    stream = _stream_for(q, k, v, o, lse, plan.ints)
+    T, H, Hkv, D, wide, narrow = _packed_shapes(q, k, plan)
+    (pq, sq), (pk, sk), (pv, sv), (po, so) = (_packed_rows("q", q, wide), _packed_rows("k", k, narrow),
+                                              _packed_rows("v", v, narrow), _packed_rows("o", o, wide))
+    d = AttnPackedDesc(pq, pk, pv, po, _packed_stat("lse", lse, H, T), None, None, None, None, None, plan.ints.data_ptr(),
+                       plan.n_seq, T, H, Hkv, D, sq, sk, sv, so, 0, 0, 0, 0, D ** -0.5 if scale is None else scale, causal)
+    check(lib().pp_attn_packed_fwd(C.byref(d), stream), "pp_attn_packed_fwd")
 
 
 def attn_packed_bwd(q, k, v, o, lse, d_o, dq, dk, dv, delta, plan: PackedPlan, *, causal: bool = True,
                     scale: Optional[float] = None) -> None:
     """Gradients of ``attn_packed_fwd``; ``delta`` fp32 [heads, rows] is a workspace."""
-    d = attn_packed_desc(q, k, v, o, lse, plan, causal, scale, d_o, dq, dk, dv, delta)
-    check(lib().pp_attn_packed_bwd(C.byref(d), current_stream()), "pp_attn_packed_bwd")
+    stream = _stream_for(q, k, v, o, lse, d_o, dq, dk, dv, delta, plan.ints)
+    T, H, Hkv, D, wide, narrow = _packed_shapes(q, k, plan)
+    (pq, sq), (pk, sk), (pv, sv), (po, so) = (_packed_rows("q", q, wide), _packed_rows("k", k, narrow),
+                                              _packed_rows("v", v, narrow), _packed_rows("o", o, wide))
+    (pdo, sdo), (pdq, sdq), (pdk, sdk), (pdv, sdv) = (_packed_rows("d_o", d_o, wide), _packed_rows("dq", dq, wide),
+                                                      _packed_rows("dk", dk, narrow), _packed_rows("dv", dv, narrow))
+    d = AttnPackedDesc(pq, pk, pv, po, _packed_stat("lse", lse, H, T), pdo, pdq, pdk, pdv,
+                       _packed_stat("delta", delta, H, T), plan.ints.data_ptr(), plan.n_seq, T, H, Hkv, D, sq, sk, sv, so,
+                       sdo, sdq, sdk, sdv, D ** -0.5 if scale is None else scale, causal)
+    check(lib().pp_attn_packed_bwd(C.byref(d), stream), "pp_attn_packed_bwd")
 
 
 # ---- embedding / loss -------------------------------------------------------------------------
