@@ -25,7 +25,7 @@ struct RouteArgs {
     const float* bias;
     int32_t E, K, n_group, topk_group;
     int32_t group_top2, renorm;
-    int32_t vec;  // rows of logits are 16-byte aligned
+    int32_t vec, vec_bias;  // rows of logits, the bias are 16-byte aligned
     float scale;
     int32_t* idx;
     float* gate;
@@ -133,7 +133,8 @@ template <typename LT, int G, int V, bool SIGMOID, bool BIASED>
 __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
     constexpr int kTokens = 256 / G, kE = G * V;
     __shared__ uint32_t gkey[kTokens][kRouteMaxGroups];
-    __shared__ uint32_t ckey[kTokens][kE];
+    __shared__ uint32_t ckey[kTokens][kE < 2 * G ? 2 * G : kE];
+    __shared__ double wide[kTokens][kRouteMaxGroups];
     __shared__ int chosen[kTokens][kRouteMaxK];
     const int tid = threadIdx.x, li = tid % G, slot = tid / G, lane = tid & 63;
     const int64_t t0 = (int64_t)blockIdx.x * kTokens + slot;
@@ -199,80 +200,113 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
         }
     }
     uint32_t key[V];
+    float bias[BIASED ? V : 1];
+    if constexpr (BIASED) {
+        if (V % 4 == 0 && a.vec_bias && e0 + V <= a.E) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+                const float4 w = reinterpret_cast<const float4*>(a.bias + e0)[i];
+                bias[4 * i] = w.x; bias[4 * i + 1] = w.y; bias[4 * i + 2] = w.z; bias[4 * i + 3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) bias[j] = e0 + j < a.E ? a.bias[e0 + j] : 0.f;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const bool there = e0 + j < a.E && x[j] != -INFINITY;
-        if constexpr (BIASED) key[j] = there ? route_key(s[j] + a.bias[e0 + j]) : 0;
+        if constexpr (BIASED) key[j] = there ? route_key(s[j] + bias[j]) : 0;
         else key[j] = there ? route_key(x[j]) : 0;
     }
 
     if (a.n_group > 1) {
         const int gs = a.E / a.n_group;
-        // sums of two rank scores (plus bias); a maximum ranks as the keys themselves do
         const bool summed = top2;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            ckey[slot][e0 + j] = key[j] == 0 ? 0 : (summed && !BIASED ? route_key(s[j]) : key[j]);
-        __syncthreads();
-        const bool open_order = BIASED || summed;  // group scores in fp32 may be out of order
-        for (int g = li; g < a.n_group; g += G) {
+        // What the group scores are made of: a maximum ranks as the keys do, sums need the choices themselves.
+        // Where every lane's experts belong to one group the lane hands on its two largest, else all of them.
+        const bool own_group = gs % V == 0;
+        const int parts = own_group ? gs / V : gs;  // entries per group
+        if (own_group) {
             uint32_t k1 = 0, k2 = 0;
-            for (int e = g * gs; e < (g + 1) * gs; ++e) {
-                const uint32_t k = ckey[slot][e];
-                if (k > k1) {
-                    k2 = k1;
-                    k1 = k;
-                } else if (k > k2) {
-                    k2 = k;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const uint32_t k = key[j] == 0 ? 0 : (summed && !BIASED ? route_key(s[j]) : key[j]);
+                const uint32_t lo = k < k1 ? k : k1;
+                k1 = k > k1 ? k : k1;
+                k2 = lo > k2 ? lo : k2;
+            }
+            ckey[slot][li] = k1;
+            ckey[slot][G + li] = k2;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                ckey[slot][e0 + j] = key[j] == 0 ? 0 : (summed && !BIASED ? route_key(s[j]) : key[j]);
+        }
+        wave_lds_fence();
+        const int n_mine = (a.n_group - li + G - 1) / G;  // groups li, li + G, ... are this lane's
+        unsigned long long open = 0;
+        uint32_t kept_min = 0xffffffffu, shut_max = 0;
+        for (int q = 0; q < n_mine; ++q) {
+            const int g = li + q * G;
+            uint32_t k1 = 0, k2 = 0;
+            for (int i = g * parts; i < (g + 1) * parts; ++i) {
+                const uint32_t k = ckey[slot][i];
+                const uint32_t lo = k < k1 ? k : k1;
+                k1 = k > k1 ? k : k1;
+                k2 = lo > k2 ? lo : k2;
+                if (own_group) {
+                    const uint32_t second = ckey[slot][G + i];
+                    k2 = second > k2 ? second : k2;
                 }
             }
             // a group with one expert left counts that one; a NaN counts as not there
             gkey[slot][g] = !summed ? (k1 > 1 ? k1 : 0) : k1 <= 1 ? 0 : k2 <= 1 ? k1 : route_key(route_value(k1) + route_value(k2));
         }
-        __syncthreads();
-        unsigned long long open = 0;
-        {
-            uint32_t kept_min = 0xffffffffu, shut_max = 0;
-            for (int g = 0; g < a.n_group; ++g) {
-                const uint32_t own = gkey[slot][g];
-                int ahead = 0;
-                for (int o = li; o < a.n_group; o += G) {
-                    const uint32_t other = gkey[slot][o];
-                    ahead += other > own || (other == own && o < g);
-                }
-                ahead = (int)route_reduce<G>((uint32_t)ahead, [](uint32_t p, uint32_t q) { return p + q; });
-                if (ahead < a.topk_group) {
-                    open |= 1ull << g;
-                    kept_min = own < kept_min ? own : kept_min;
-                } else {
-                    shut_max = own > shut_max ? own : shut_max;
-                }
+        wave_lds_fence();
+        for (int q = 0; q * G < a.n_group; ++q) {
+            const int g = li + q * G;
+            const uint32_t own = g < a.n_group ? gkey[slot][g] : 0;
+            int ahead = 0;
+#pragma unroll 8
+            for (int o = 0; o < a.n_group; ++o) {
+                const uint32_t other = gkey[slot][o];
+                ahead += other > own || (other == own && o < g);
             }
+            const bool kept = g < a.n_group && ahead < a.topk_group;
+            open |= ((__ballot(kept) & mine) >> (lane & ~(G - 1))) << (q * G);
+            if (kept) kept_min = own < kept_min ? own : kept_min;
+            else if (g < a.n_group) shut_max = own > shut_max ? own : shut_max;
+        }
+        // group scores in fp32 whose order is open, at the border: again in 64 bits, from the members that may be
+        // the largest (each member is off by half a margin, the sum of two by one)
+        if (BIASED || summed) {
+            kept_min = route_min<G>(kept_min);
+            shut_max = route_max<G>(shut_max);
             bool doubt = false;
-            if (open_order && shut_max > 1 && kept_min > 1) {
+            if (shut_max > 1 && kept_min > 1) {
                 const float hi = route_value(kept_min), lo = route_value(shut_max);
                 doubt = hi - lo <= 2.0f * route_margin<SIGMOID>(s_max, fmaxf(fabsf(hi), fabsf(lo)));
             }
-            // (the threshold of a group's two best members is below: their own margins count too)
             if (__any(doubt)) {
-                // the group scores again in 64 bits, from the members that may be the two largest
                 const double total = SIGMOID ? 1.0 : route_sum64<LT, G>(a, t, li, m);
-                __shared__ double wide[kTokens][kRouteMaxGroups];
-                for (int g = li; g < a.n_group; g += G) {
+                wave_lds_fence();
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    ckey[slot][e0 + j] = key[j] == 0 ? 0 : (summed && !BIASED ? route_key(s[j]) : key[j]);
+                wave_lds_fence();
+                for (int q = 0; q < n_mine; ++q) {
+                    const int g = li + q * G;
                     uint32_t k1 = 0, k2 = 0;
                     for (int e = g * gs; e < (g + 1) * gs; ++e) {
                         const uint32_t k = ckey[slot][e];
-                        if (k > k1) {
-                            k2 = k1;
-                            k1 = k;
-                        } else if (k > k2) {
-                            k2 = k;
-                        }
+                        const uint32_t lo = k < k1 ? k : k1;
+                        k1 = k > k1 ? k : k1;
+                        k2 = lo > k2 ? lo : k2;
                     }
-                    const uint32_t least = summed && k2 > 1 ? k2 : k1;
                     double b1 = -INFINITY, b2 = -INFINITY;
                     if (k1 > 1) {
-                        const float v = route_value(least);
+                        const float v = route_value(summed && k2 > 1 ? k2 : k1);
                         const uint32_t from = route_key(v - route_margin<SIGMOID>(s_max, v));
                         for (int e = g * gs; e < (g + 1) * gs; ++e) {
                             if (ckey[slot][e] <= 1 || ckey[slot][e] < from) continue;
@@ -299,9 +333,15 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
                 if (doubt) open = again;
             }
         }
+        int g = e0 / gs, left = (g + 1) * gs - e0;  // group of the expert, experts up to its end
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (e0 + j < a.E && !((open >> ((e0 + j) / gs)) & 1)) key[j] = 0;
+        for (int j = 0; j < V; ++j) {
+            if (e0 + j < a.E && !((open >> g) & 1)) key[j] = 0;
+            if (--left == 0) {
+                ++g;
+                left = gs;
+            }
+        }
     }
 
     for (int k = 0; k < a.K; ++k) {
@@ -329,8 +369,13 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
                 double c = -INFINITY;
                 for (uint32_t left = top > 1 ? cand : 0; left; left &= left - 1) {
                     const int j = __ffs(left) - 1;
-                    const double w = route_score64<SIGMOID>(route_load<LT>(a.logits, t * a.ld + e0 + j), m, total) +
-                                     (double)a.bias[e0 + j];
+                    float xj = x[0], bj = bias[0];
+#pragma unroll
+                    for (int i = 1; i < V; ++i) {
+                        xj = i == j ? x[i] : xj;
+                        bj = i == j ? bias[i] : bj;
+                    }
+                    const double w = route_score64<SIGMOID>(xj, m, total) + (double)bj;
                     if (w > c) {
                         c = w;
                         at = j;
@@ -718,6 +763,7 @@ extern "C" int pp_moe_route(const pp_moe_route_desc* d, pp_stream stream) {
     const int64_t size = d->dtype == PP_BF16 ? 2 : 4;
     a.group_top2 = d->group_score == PP_MOE_GROUP_TOP2;
     a.vec = aligned(d->logits, 16) && d->ld * size % 16 == 0;
+    a.vec_bias = aligned(d->bias, 16);
     const bool sig = d->scoring == PP_MOE_SIGMOID, biased = d->bias != nullptr;
     if (d->dtype == PP_BF16) {
         if (sig) return biased ? route_launch<uint16_t, true, true>(a, st) : route_launch<uint16_t, true, false>(a, st);
