@@ -33,6 +33,7 @@ struct PackedArgs {
     int64_t T;
     int32_t H, G;       // query heads; query heads per key / value head
     const int32_t* plan;
+    int32_t cap64;      // entries that the plan reserves for blocks of 64 rows
     float scale;
 };
 
@@ -144,9 +145,10 @@ struct PackedTileLoader {
         }
     }
     __device__ __forceinline__ void load(uint16_t* lds, int row0, int wave, int64_t extra = 0) const {
-        const int left = len - row0;
+        const int left = len - row0;  // none: a resource of no bytes, everything reads as zeros
         const __amdgpu_buffer_rsrc_t rsrc =
-            make_rsrc(base + (int64_t)row0 * stride + extra, (uint64_t)(left < 64 ? left : 64) * (uint64_t)stride * 2);
+            make_rsrc(base + (int64_t)row0 * stride + extra,
+                      left <= 0 ? 0 : (uint64_t)(left < 64 ? left : 64) * (uint64_t)stride * 2);
 #pragma unroll
         for (int s = 0; s < DS; ++s)
 #pragma unroll
@@ -299,7 +301,176 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(c
     if (lh == 0) a.lse[(int64_t)w.h * a.T + w.row0 + qi] = m * a.scale + logf(l);
 }
 
+// The form for long sequences: a work-group owns 128 query rows, 32 per wave, and every wave walks all keys, in
+// blocks of 64: twice the products per staged block and barrier, half the passes over keys and values, and no merge.
+template <int D, bool CAUSAL>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd128_kernel(const PackedArgs a) {
+    constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
+    constexpr int kOperand = DS * kTile, kStage = 2 * kOperand;
+    uint16_t* const lds = attn_lds;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, lh = lane >> 5;
+    PackedBlock w;
+    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader) + a.cap64, a.plan[1], &w)) return;
+    const int q0 = w.j * 128, qw0 = q0 + 32 * wave, qi = qw0 + l32;
+    const int hk = w.h / a.G;
+
+    PackedTileLoader<DS> lk, lv;
+    lk.init(a.k + w.row0 * a.sk + (int64_t)hk * D, a.sk, w.len, wave, lane);
+    lv.init(a.v + w.row0 * a.sv + (int64_t)hk * D, a.sv, w.len, wave, lane);
+    const int n_keys = CAUSAL && q0 + 128 < w.len ? q0 + 128 : w.len;
+    const int n_blocks = (n_keys + 63) / 64;
+    auto issue = [&](int stage, int j) {
+        lk.load(lds + stage * kStage, j * 64, wave);
+        lv.load(lds + stage * kStage + kOperand, j * 64, wave);
+    };
+
+    const int qr = qi < w.len ? qi : w.len - 1;
+    const uint16_t* qp = a.q + (w.row0 + qr) * a.sq + (int64_t)w.h * D;
+    bf16x8_t qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * ks + 8 * lh);
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t)
+        if (t < n_blocks) issue(t, t);
+
+    f32x16_t oacc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[t][e] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    const float c = a.scale * kLog2e;
+    const int partner = (lane ^ 32) << 2;
+    // keys that some query of this wave sees
+    const int seen = CAUSAL && qw0 + 32 < w.len ? qw0 + 32 : w.len;
+
+    // N tiles of 32 keys from key kt0 on, tile rows kr ..; MASKED: keys past the last visible one are left out
+    auto step = [&](auto n_c, auto masked_c, const uint16_t* Ks, const uint16_t* Vs, int kr, int kt0)
+        __attribute__((always_inline)) {
+        constexpr int N = decltype(n_c)::value;
+        f32x16_t s[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int t = 0; t < N; ++t) {
+                const bf16x8_t kf = read_row_frag(Ks + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], s[t], 0, 0, 0);
+            }
+        if constexpr (decltype(masked_c)::value) {
+            const int lim = (CAUSAL ? qr : w.len - 1) - kt0 - 4 * lh;
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (32 * t + 8 * (v >> 2) + (v & 3) > lim) s[t][v] = -INFINITY;
+        }
+        float mloc = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) mloc = fmaxf(mloc, s[t][v]);
+        if (__ballot(mloc * c > m_run * c + 8.0f)) {
+            mloc = fmaxf(mloc, __int_as_float(__builtin_amdgcn_ds_bpermute(partner, __float_as_int(mloc))));
+            const float m_new = fmaxf(m_run, mloc);
+            const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m_run - m_new) * c);
+            l_run *= alpha;
+            m_run = m_new;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[t][e] *= alpha;
+        }
+        const float mc = (m_run == -INFINITY ? 0.f : m_run) * c;
+        float psum = 0.f;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                s[t][v] = __builtin_amdgcn_exp2f(fmaf(s[t][v], c, -mc));
+                psum += s[t][v];
+            }
+        l_run += psum;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int gp = 0; gp < 2; ++gp) {
+                float pv[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pv[e] = s[t][8 * gp + e];
+                const bf16x8_t pb = pack8(pv);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const bf16x8_t vf = read_col_frag(Vs + (dt / 2) * kTile, kr + 32 * t + 16 * gp, 32 * (dt % 2), lane);
+                    oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, oacc[dt], 0, 0, 0);
+                }
+            }
+    };
+    // Blocks that every query of the work-group sees whole, NS at a time (stages and LDS addresses are constants),
+    // without any masking code; then what is left, one tile of 32 keys at a time.
+    const int n_whole = (CAUSAL && q0 < w.len ? q0 : w.len) / 64;
+    int j = 0;
+    for (; j + NS <= n_whole; j += NS)
+        static_for<NS>([&](auto stage_c) __attribute__((always_inline)) {
+            constexpr int stage = decltype(stage_c)::value;
+            await_block<4 * DS, NS>(j + stage, n_blocks);
+            if (j + stage + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + stage + NS - 1);
+            step(std::integral_constant<int, 2>{}, std::false_type{}, lds + stage * kStage, lds + stage * kStage + kOperand,
+                 0, (j + stage) * 64);
+        });
+    for (int stage = 0; j < n_blocks; ++j) {
+        await_block<4 * DS, NS>(j, n_blocks);
+        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
+        for (int t = 0; t < 2; ++t)
+            if (j * 64 + 32 * t < seen)
+                step(std::integral_constant<int, 1>{}, std::true_type{}, lds + stage * kStage,
+                     lds + stage * kStage + kOperand, 32 * t, j * 64 + 32 * t);
+        stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+    l_run += __int_as_float(__builtin_amdgcn_ds_bpermute(partner, __float_as_int(l_run)));
+    if (qi >= w.len) return;
+    const float inv_l = 1.0f / l_run;
+    uint16_t* op = a.o + (w.row0 + qi) * a.so + (int64_t)w.h * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = oacc[dt][4 * g + e] * inv_l;
+            const int d = 32 * dt + 8 * g + 4 * lh;
+            *reinterpret_cast<uint2*>(op + d) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+        }
+    if (lh == 0) a.lse[(int64_t)w.h * a.T + w.row0 + qi] = m_run * a.scale + logf(l_run);
+}
+
 // ---- backward: dQ -------------------------------------------------------------------------------
+// Fragments of a lane's query row, and delta = rowsum(dO * O) (the lane pair lh = 0, 1 holds the row).
+template <int KS>
+__device__ __forceinline__ float packed_delta(const uint16_t* qp, const uint16_t* dop, const uint16_t* op, int lh,
+                                              bf16x8_t (&qf)[KS], bf16x8_t (&dof)[KS]) {
+    float delta = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * ks + 8 * lh);
+        dof[ks] = *reinterpret_cast<const bf16x8_t*>(dop + 16 * ks + 8 * lh);
+        Frag x, y;
+        x.v = dof[ks];
+        y.u = *reinterpret_cast<const uint4*>(op + 16 * ks + 8 * lh);
+        delta += bf16lo(x.u.x) * bf16lo(y.u.x) + bf16hi(x.u.x) * bf16hi(y.u.x) +
+                 bf16lo(x.u.y) * bf16lo(y.u.y) + bf16hi(x.u.y) * bf16hi(y.u.y) +
+                 bf16lo(x.u.z) * bf16lo(y.u.z) + bf16hi(x.u.z) * bf16hi(y.u.z) +
+                 bf16lo(x.u.w) * bf16lo(y.u.w) + bf16hi(x.u.w) * bf16hi(y.u.w);
+    }
+    return delta + __shfl_xor(delta, 32, 64);
+}
+
 // A work-group owns 64 query rows (2 groups of 32 queries x 2 halves of every key block) and hands the dK / dV
 // kernel the row sums D = sum_j P dP.
 template <int D, bool CAUSAL>
@@ -331,21 +502,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
     const uint16_t* dop = a.d_o + row * a.sdo + (int64_t)w.h * D;
     const uint16_t* op = a.o + row * a.so + (int64_t)w.h * D;
     bf16x8_t qf[KS], dof[KS];
-    // delta = rowsum(dO * O): the lane pair (lh = 0, 1) holds the row
-    float delta_q = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * ks + 8 * lh);
-        dof[ks] = *reinterpret_cast<const bf16x8_t*>(dop + 16 * ks + 8 * lh);
-        Frag x, y;
-        x.v = dof[ks];
-        y.u = *reinterpret_cast<const uint4*>(op + 16 * ks + 8 * lh);
-        delta_q += bf16lo(x.u.x) * bf16lo(y.u.x) + bf16hi(x.u.x) * bf16hi(y.u.x) +
-                   bf16lo(x.u.y) * bf16lo(y.u.y) + bf16hi(x.u.y) * bf16hi(y.u.y) +
-                   bf16lo(x.u.z) * bf16lo(y.u.z) + bf16hi(x.u.z) * bf16hi(y.u.z) +
-                   bf16lo(x.u.w) * bf16lo(y.u.w) + bf16hi(x.u.w) * bf16hi(y.u.w);
-    }
-    delta_q += __shfl_xor(delta_q, 32, 64);
+    const float delta_q = packed_delta<KS>(qp, dop, op, lh, qf, dof);
     const float lse_q = a.lse[(int64_t)w.h * a.T + row] * kLog2e;
     // The sum of P dP over the keys equals delta in exact arithmetic and is the one under which the rows of dS
     // sum to zero; it is complete only behind the loop and is what the dK / dV kernel gets.
@@ -436,12 +593,142 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         }
 }
 
+// The form for long sequences: 128 query rows, 32 per wave, every wave over all keys (see the forward).
+template <int D, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const PackedArgs a) {
+    constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
+    constexpr int kOperand = DS * kTile, kStage = 2 * kOperand;
+    uint16_t* const lds = attn_lds;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, lh = lane >> 5;
+    PackedBlock w;
+    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader) + a.cap64, a.plan[1], &w)) return;
+    const int q0 = w.j * 128, qw0 = q0 + 32 * wave, qi = qw0 + l32;
+    const int hk = w.h / a.G;
+
+    PackedTileLoader<DS> lk, lv;
+    lk.init(a.k + w.row0 * a.sk + (int64_t)hk * D, a.sk, w.len, wave, lane);
+    lv.init(a.v + w.row0 * a.sv + (int64_t)hk * D, a.sv, w.len, wave, lane);
+    const int n_keys = CAUSAL && q0 + 128 < w.len ? q0 + 128 : w.len;
+    const int n_blocks = (n_keys + 63) / 64;
+    auto issue = [&](int stage, int j) {
+        lk.load(lds + stage * kStage, j * 64, wave);
+        lv.load(lds + stage * kStage + kOperand, j * 64, wave);
+    };
+
+    const int qr = qi < w.len ? qi : w.len - 1;
+    const int64_t row = w.row0 + qr;
+    const uint16_t* qp = a.q + row * a.sq + (int64_t)w.h * D;
+    const uint16_t* dop = a.d_o + row * a.sdo + (int64_t)w.h * D;
+    const uint16_t* op = a.o + row * a.so + (int64_t)w.h * D;
+    bf16x8_t qf[KS], dof[KS];
+    const float delta_q = packed_delta<KS>(qp, dop, op, lh, qf, dof);
+    const float lse_q = a.lse[(int64_t)w.h * a.T + row] * kLog2e;
+    float d_sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t)
+        if (t < n_blocks) issue(t, t);
+    const float c = a.scale * kLog2e;
+    const int seen = CAUSAL && qw0 + 32 < w.len ? qw0 + 32 : w.len;
+
+    f32x16_t dqacc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dqacc[t][e] = 0.f;
+
+    auto step = [&](auto n_c, auto masked_c, const uint16_t* Ks, const uint16_t* Vs, int kr, int kt0)
+        __attribute__((always_inline)) {
+        constexpr int N = decltype(n_c)::value;
+        f32x16_t s[N], dp[N];
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[t][e] = 0.f;
+                dp[t][e] = 0.f;
+            }
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const bf16x8_t kfr = read_row_frag(Ks + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
+                const bf16x8_t vfr = read_row_frag(Vs + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr, qf[ks], s[t], 0, 0, 0);
+                dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr, dof[ks], dp[t], 0, 0, 0);
+            }
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[t][v] = __builtin_amdgcn_exp2f(fmaf(s[t][v], c, -lse_q));
+            if constexpr (decltype(masked_c)::value) {
+                const int lim = (CAUSAL ? qr : w.len - 1) - kt0 - 4 * lh;
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (32 * t + 8 * (v >> 2) + (v & 3) > lim) s[t][v] = 0.f;
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v) d_sum = fmaf(s[t][v], dp[t][v], d_sum);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[t][v] *= dp[t][v] - delta_q;
+#pragma unroll
+            for (int gp = 0; gp < 2; ++gp) {
+                float ds[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ds[e] = s[t][8 * gp + e];
+                const bf16x8_t dsb = pack8(ds);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const bf16x8_t ktf = read_col_frag(Ks + (dt / 2) * kTile, kr + 32 * t + 16 * gp, 32 * (dt % 2), lane);
+                    dqacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktf, dsb, dqacc[dt], 0, 0, 0);
+                }
+            }
+        }
+    };
+    const int n_whole = (CAUSAL && q0 < w.len ? q0 : w.len) / 64;
+    int j = 0;
+    for (; j + NS <= n_whole; j += NS)
+        static_for<NS>([&](auto stage_c) __attribute__((always_inline)) {
+            constexpr int stage = decltype(stage_c)::value;
+            await_block<4 * DS, NS>(j + stage, n_blocks);
+            if (j + stage + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + stage + NS - 1);
+            step(std::integral_constant<int, 2>{}, std::false_type{}, lds + stage * kStage, lds + stage * kStage + kOperand,
+                 0, (j + stage) * 64);
+        });
+    for (int stage = 0; j < n_blocks; ++j) {
+        await_block<4 * DS, NS>(j, n_blocks);
+        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
+        for (int t = 0; t < 2; ++t)
+            if (j * 64 + 32 * t < seen)
+                step(std::integral_constant<int, 1>{}, std::true_type{}, lds + stage * kStage,
+                     lds + stage * kStage + kOperand, 32 * t, j * 64 + 32 * t);
+        stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+    d_sum += __shfl_xor(d_sum, 32, 64);
+    if (qi >= w.len) return;
+    if (lh == 0) a.delta[(int64_t)w.h * a.T + row] = d_sum;
+    uint16_t* dqp = a.dq + row * a.sdq + (int64_t)w.h * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = dqacc[dt][4 * g + e] * a.scale;
+            const int d = 32 * dt + 8 * g + 4 * lh;
+            *reinterpret_cast<uint2*>(dqp + d) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+        }
+}
+
 // ---- backward: dK, dV ---------------------------------------------------------------------------
 // A work-group owns 64 keys of one key / value head and walks the query blocks that see them, one query head of
 // the group after the other, so the sums over a group have a fixed order.  4 waves: 2 groups of 32 keys x 2
-// halves of every query block.
-template <int D, bool CAUSAL>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 1) void attn_packed_bwd_dkv_kernel(const PackedArgs a) {
+// halves of every query block.  Head dimension 64.
+template <bool CAUSAL>
+__global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const PackedArgs a) {
+    constexpr int D = 64;
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
     constexpr int kOperand = DS * kTile;
     constexpr int kStage = 2 * kOperand + 256;  // Q, dO, 64 lse, 64 delta
@@ -508,18 +795,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void attn_packed_bwd_dkv_kern
         }
     const float c = a.scale * kLog2e;
 
-    int stage = 0, cur_b = 0;
-    for (int j = 0; j < nb; ++j) {
-        const int qt0 = (jq0 + cur_b) * 64 + 32 * half;
-        cur_b = cur_b + 1 == nb_head ? 0 : cur_b + 1;
-        await_block<4 * DS + 1, NS>(j, nb);
-        if (j + NS - 1 < nb) issue(stage == 0 ? NS - 1 : stage - 1);
-        const uint16_t* Qs = lds + stage * kStage;
+    // one block of 64 queries from query qb0 on; MASKED: the diagonal block of a causal mask
+    auto step = [&](auto masked_c, const uint16_t* Qs, int qb0) __attribute__((always_inline)) {
         const uint16_t* Os = Qs + kOperand;
         const float* lse_s = reinterpret_cast<const float*>(Qs + 2 * kOperand);
         const float* delta_s = lse_s + 64;
-        stage = stage + 1 == NS ? 0 : stage + 1;
-        if (qt0 >= w.len || (CAUSAL && qt0 + 31 < kvw0)) continue;  // every query precedes every key
         f32x16_t sacc, dpacc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -533,8 +813,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void attn_packed_bwd_dkv_kern
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qfr, kf[ks], sacc, 0, 0, 0);
             dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ofr, vf[ks], dpacc, 0, 0, 0);
         }
-        // element v: query qt0 + 8 (v / 4) + 4 lh + v % 4, key kvi.  A query past the end has zero rows, a zero
-        // log-sum-exp and a zero delta: P = 1 meets dO = 0, dS = 0.
+        // element v: query qb0 + 32 half + 8 (v / 4) + 4 lh + v % 4, key kvi.  A query past the end has zero rows, a
+        // zero log-sum-exp and a zero delta: P = 1 meets dO = 0, dS = 0.
         float pv[16], dsv[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -544,10 +824,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void attn_packed_bwd_dkv_kern
             for (int e = 0; e < 4; ++e)
                 pv[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sacc[4 * g + e], c, -lq4[e]));
         }
-        if (CAUSAL && qt0 < kvw0 + 31) {
+        if constexpr (decltype(masked_c)::value) {
+            const int lim = kvi - qb0 - 32 * half - 4 * lh;  // earlier queries do not see this key
 #pragma unroll
             for (int v = 0; v < 16; ++v)
-                if (kvi > qt0 + 8 * (v >> 2) + 4 * lh + (v & 3)) pv[v] = 0.f;
+                if (8 * (v >> 2) + (v & 3) < lim) pv[v] = 0.f;
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -568,6 +849,24 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void attn_packed_bwd_dkv_kern
                 dkacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtf, dsb, dkacc[dt], 0, 0, 0);
             }
         }
+    };
+    int stage = 0, j = 0;
+    auto next = [&]() __attribute__((always_inline)) {
+        await_block<4 * DS + 1, NS>(j, nb);
+        if (j + NS - 1 < nb) issue(stage == 0 ? NS - 1 : stage - 1);
+        const uint16_t* Qs = lds + stage * kStage;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        ++j;
+        return Qs;
+    };
+    // per query head of the group: the diagonal block, then blocks without any masking code
+    for (int g = 0; g < a.G; ++g) {
+        int b = 0;
+        if constexpr (CAUSAL) {
+            step(std::true_type{}, next(), jq0 * 64);
+            b = 1;
+        }
+        for (; b < nb_head; ++b) step(std::false_type{}, next(), 0);
     }
     // add the sums of the two halves: [grp][16 DT values][64 lanes] floats, dV then dK
     wait_lds();
@@ -600,6 +899,204 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 1) void attn_packed_bwd_dkv_kern
         __syncthreads();
     }
 }
+
+// Head dimension 128: 8 waves per work-group, so that two waves share a SIMD and one's products run beside the
+// other's exponentials; to fit the registers of that the value rows stay in LDS.  KB blocks of 64 keys per
+// work-group: 2, as 4 groups of 32 keys x 2 parts of a step of 64 queries, or 1, as 2 groups x 4 parts of 128
+// queries: twice the work-groups with half the steps each, for launches that would not fill the CUs.
+template <int D, bool CAUSAL, int KB>
+__global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const PackedArgs a) {
+    constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = 2;
+    constexpr int GROUPS = 2 * KB, PARTS = 8 / GROUPS, QB = PARTS / 2;  // QB: blocks of 64 queries per step
+    constexpr int kOperand = DS * kTile;                  // a block of 64 rows
+    constexpr int kStats = 2 * QB * kOperand;             // Q blocks, dO blocks, then 64 QB lse, 64 QB delta
+    constexpr int kStage = kStats + 256 * QB;
+    uint16_t* const lds = attn_lds;
+    uint16_t* const Vl = lds + NS * kStage;               // [KB blocks of 64 keys][DS] tiles
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave % GROUPS, part = wave / GROUPS;
+    const int set = wave >> 2, lwave = wave & 3;          // waves 0-3 load Q, waves 4-7 dO
+    const int l32 = lane & 31, lh = lane >> 5;
+    PackedBlock w;  // w.h: key / value head
+    if (!packed_block_of(a, a.H / a.G, reinterpret_cast<const int4*>(a.plan + kPlanHeader) + (KB == 2 ? a.cap64 : 0),
+                         a.plan[KB - 1], &w))
+        return;
+    // the plan's order is by query work; under a causal mask key blocks count from the end (see above)
+    const int jk = CAUSAL ? (w.len + 64 * KB - 1) / (64 * KB) - 1 - w.j : w.j;
+    const int kv0 = jk * (64 * KB), kvi = kv0 + 32 * grp + l32;
+    const int h0 = w.h * a.G;
+
+    PackedTileLoader<DS> lx;
+    if (set == 0) lx.init(a.q + w.row0 * a.sq + (int64_t)h0 * D, a.sq, w.len, lwave, lane);
+    else lx.init(a.d_o + w.row0 * a.sdo + (int64_t)h0 * D, a.sdo, w.len, lwave, lane);
+    const float* stat = (set ? a.delta : a.lse) + (int64_t)h0 * a.T + w.row0;
+
+    constexpr int kStep = 64 * QB;                        // queries per step
+    const int u0 = CAUSAL ? kv0 / kStep : 0;              // first step that sees these keys
+    const int n_head = (w.len + kStep - 1) / kStep - u0, nb = a.G * n_head;
+    int iss_g = 0, iss_b = 0;
+    auto issue = [&](int stage) {  // steps are issued in order
+        uint16_t* st = lds + stage * kStage;
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+            const int row0 = (u0 + iss_b) * kStep + 64 * q;
+            // a block past the end loads nothing but zeros, through a resource of no bytes
+            lx.load(st + (set * QB + q) * kOperand, row0, lwave, (int64_t)iss_g * D);
+            const int left = w.len - row0;
+            const __amdgpu_buffer_rsrc_t rs =
+                make_rsrc(stat + (int64_t)iss_g * a.T + row0, left <= 0 ? 0 : (uint64_t)(left < 64 ? left : 64) * 4);
+            // (every wave of a set the same values: the same number of loads outstanding in each)
+            load_floats_to_lds(rs, reinterpret_cast<float*>(st + kStats) + (set * QB + q) * 64, 0, lane);
+        }
+        if (++iss_b == n_head) {
+            iss_b = 0;
+            ++iss_g;
+        }
+    };
+
+    const int64_t krow = w.row0 + (kvi < w.len ? kvi : w.len - 1);
+    const uint16_t* kp = a.k + krow * a.sk + (int64_t)w.h * D;
+    bf16x8_t kf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const bf16x8_t*>(kp + 16 * ks + 8 * lh);
+    if (set < KB) {  // a set of four waves per block of 64 keys
+        PackedTileLoader<DS> lv;
+        lv.init(a.v + w.row0 * a.sv + (int64_t)w.h * D, a.sv, w.len, lwave, lane);
+        lv.load(Vl + set * kOperand, kv0 + 64 * set, lwave);
+    }
+    if (nb > 0) issue(0);
+
+    f32x16_t dvacc[DT], dkacc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            dvacc[t][e] = 0.f;
+            dkacc[t][e] = 0.f;
+        }
+    const float c = a.scale * kLog2e;
+    const uint16_t* Vs = Vl + (grp >> 1) * kOperand;
+    const int vrow = 32 * (grp & 1) + l32;
+    const int qblk = part >> 1, half = part & 1;          // this wave's 32 queries of a step
+
+    auto step = [&](auto masked_c, const uint16_t* st, int qb0) __attribute__((always_inline)) {
+        const uint16_t* Qs = st + qblk * kOperand;
+        const uint16_t* Os = st + (QB + qblk) * kOperand;
+        const float* lse_s = reinterpret_cast<const float*>(st + kStats) + 64 * qblk + 32 * half + 4 * lh;
+        const float* delta_s = lse_s + 64 * QB;
+        f32x16_t sacc, dpacc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sacc[e] = 0.f;
+            dpacc[e] = 0.f;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8_t qfr = read_row_frag(Qs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qfr, kf[ks], sacc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8_t ofr = read_row_frag(Os + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t vfr = read_row_frag(Vs + (ks / 4) * kTile, vrow, 2 * (ks % 4) + lh);
+            dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ofr, vfr, dpacc, 0, 0, 0);
+        }
+        float pv[16], dsv[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 l4 = *reinterpret_cast<const float4*>(lse_s + 8 * g);
+            const float lq4[4] = {l4.x * kLog2e, l4.y * kLog2e, l4.z * kLog2e, l4.w * kLog2e};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                pv[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sacc[4 * g + e], c, -lq4[e]));
+        }
+        if constexpr (decltype(masked_c)::value) {
+            const int lim = kvi - qb0 - 32 * part - 4 * lh;  // earlier queries do not see this key
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (8 * (v >> 2) + (v & 3) < lim) pv[v] = 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 d4 = *reinterpret_cast<const float4*>(delta_s + 8 * g);
+            const float dq4[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dsv[4 * g + e] = pv[4 * g + e] * (dpacc[4 * g + e] - dq4[e]);
+        }
+#pragma unroll
+        for (int gp = 0; gp < 2; ++gp) {
+            const bf16x8_t pb = pack8(pv + 8 * gp);
+            const bf16x8_t dsb = pack8(dsv + 8 * gp);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const bf16x8_t otf = read_col_frag(Os + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t qtf = read_col_frag(Qs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                dvacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(otf, pb, dvacc[dt], 0, 0, 0);
+                dkacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtf, dsb, dkacc[dt], 0, 0, 0);
+            }
+        }
+    };
+    int stage = 0, j = 0;
+    auto next = [&]() __attribute__((always_inline)) {
+        await_block<QB * (2 * DS + 1), NS>(j, nb);
+        if (j + 1 < nb) issue(stage ^ 1);
+        const uint16_t* st = lds + stage * kStage;
+        stage ^= 1;
+        ++j;
+        return st;
+    };
+    // per query head of the group: the steps that the diagonal crosses, then steps without any masking code
+    constexpr int kDiag = CAUSAL ? KB / QB > 1 ? KB / QB : 1 : 0;
+    for (int g = 0; g < a.G; ++g) {
+        int b = 0;
+        for (; b < kDiag && b < n_head; ++b) step(std::true_type{}, next(), (u0 + b) * kStep);
+        for (; b < n_head; ++b) step(std::false_type{}, next(), 0);
+    }
+    // add the sums of the parts in a fixed order: [part - 1][grp][16 DT values][64 lanes] floats, dV then dK
+    wait_lds();
+    __syncthreads();
+    float* xs = reinterpret_cast<float*>(lds) + grp * (16 * DT * 64) + lane;
+    constexpr int kPart = GROUPS * 16 * DT * 64;
+    static_assert((PARTS - 1) * kPart * 4 <= NS * kStage * 2, "the exchange fits the stages");
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+        f32x16_t(&acc)[DT] = pass == 0 ? dvacc : dkacc;
+        if (part != 0) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) xs[(part - 1) * kPart + (16 * dt + e) * 64] = acc[dt][e];
+        }
+        __syncthreads();
+        if (part == 0 && kvi < w.len) {
+            uint16_t* outp = (pass == 0 ? a.dv + krow * a.sdv : a.dk + krow * a.sdk) + (int64_t)w.h * D;
+            const float f = pass == 0 ? 1.0f : a.scale;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float s[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[e] = acc[dt][4 * g + e];
+#pragma unroll
+                        for (int q = 0; q < PARTS - 1; ++q) s[e] += xs[q * kPart + (16 * dt + 4 * g + e) * 64];
+                        s[e] *= f;
+                    }
+                    const int d = 32 * dt + 8 * g + 4 * lh;
+                    *reinterpret_cast<uint2*>(outp + d) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
+                }
+        }
+        __syncthreads();
+    }
+}
+
+static constexpr size_t dkv8_lds_bytes(int D, int kb) {
+    return (size_t)2 * ((2 / kb) * (2 * (D / 64) * kTile * 2 + 512)) + (size_t)kb * (D / 64) * kTile * 2;
+}
+static_assert(dkv8_lds_bytes(128, 1) <= 160 * 1024 && dkv8_lds_bytes(128, 2) <= 160 * 1024, "a work-group's LDS");
 
 // ---- entry points -------------------------------------------------------------------------------
 static int packed_check(const char* who, const pp_attn_packed_desc* d, bool bwd) {
@@ -644,43 +1141,78 @@ static PackedArgs packed_args(const pp_attn_packed_desc* d) {
     a.H = (int32_t)d->H;
     a.G = (int32_t)(d->H / d->Hkv);
     a.plan = d->plan;
+    a.cap64 = (int32_t)plan_blocks64(d->T, d->n_seq);
     a.scale = d->scale;
     return a;
 }
 
-// Dynamic LDS: the stages, or the exchange buffers of the epilogue if those are larger.
-static size_t packed_lds_bytes(int D, bool dkv) {
-    const size_t stages = (size_t)attn_stages(D) * ((size_t)2 * (D / 64) * kTile * 2 + (dkv ? 512 : 0));
-    const size_t merge = (size_t)2 * (16 * (D / 32) + 2) * 64 * 4;
-    return stages > merge ? stages : merge;
+// Dynamic LDS of the forward and dQ kernels: the stages (the exchange of the epilogue is smaller).
+static size_t packed_lds_bytes(int D) {
+    return (size_t)attn_stages(D) * 2 * (D / 64) * kTile * 2;
 }
+static_assert(3 * 2 * kTile * 2 >= 2 * (16 * 2 + 2) * 64 * 4 && 2 * 2 * 2 * kTile * 2 >= 2 * (16 * 4 + 2) * 64 * 4,
+              "the exchange of two halves fits the stages");
 
 template <auto kernel>
-static int packed_launch(const char* name, int64_t grid, size_t lds, hipStream_t st, const PackedArgs& a) {
+static int packed_launch(const char* name, int threads, int64_t grid, size_t lds, hipStream_t st, const PackedArgs& a) {
+    // one attribute call per kernel (the kernel is a template argument, so is the static) and process
     static const hipError_t attr_rc =
         hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (attr_rc != hipSuccess)
         return fail(PP_ERR_LAUNCH, "%s: cannot reserve %zu bytes of LDS: %s", name, lds, hipGetErrorString(attr_rc));
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(256), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), lds, st, a);
     return check_launch(name);
+}
+
+// 128-row forms where the launch has at least as many blocks of 128 rows as the CUs hold work-groups at once (3 of
+// head dimension 64, 2 of 128; the sequences' last, partly filled blocks are left out of the count).  With fewer,
+// half as many work-groups leave CUs idle and the last one takes twice as long.  Forward, us, 64 rows | 128 rows:
+//   D = 64:  [16 heads] T = 2048: 23.7 | 27.6, 4096: 50.6 | 57.4; [12 heads] T = 8192: 150 | 129; [16] T = 16384 in 16
+//            sequences: 89.6 | 74.4, in 256: 42.8 | 39.1
+//   D = 128: [32 heads] T = 1024: 20.7 | 24.3, 2048: 50.6 | 49.7, 4096: 169 | 141, 16384 in 3 sequences: 1070 | 870
+// The backward's dQ takes it for D = 128 only (T = 16384, 16 heads of 64: 290 us against 306 for the whole backward).
+static bool packed_wide(const pp_attn_packed_desc* d, int64_t heads) {
+    return d->T / 128 * heads >= (d->D == 64 ? 3 : 2) * 256;
 }
 
 template <int D, bool CAUSAL>
 static int packed_fwd(const pp_attn_packed_desc* d, hipStream_t st) {
-    return packed_launch<attn_packed_fwd_kernel<D, CAUSAL>>("attn_packed_fwd_kernel", plan_blocks64(d->T, d->n_seq) * d->H,
-                                                            packed_lds_bytes(D, false), st, packed_args(d));
+    const PackedArgs a = packed_args(d);
+    const size_t lds = packed_lds_bytes(D);
+    if (packed_wide(d, d->H))
+        return packed_launch<attn_packed_fwd128_kernel<D, CAUSAL>>("attn_packed_fwd128_kernel", 256,
+                                                                   plan_blocks128(d->T, d->n_seq) * d->H, lds, st, a);
+    return packed_launch<attn_packed_fwd_kernel<D, CAUSAL>>("attn_packed_fwd_kernel", 256,
+                                                            plan_blocks64(d->T, d->n_seq) * d->H, lds, st, a);
 }
 
 template <int D, bool CAUSAL>
 static int packed_bwd(const pp_attn_packed_desc* d, hipStream_t st) {
     const PackedArgs a = packed_args(d);
-    const int64_t blocks = plan_blocks64(d->T, d->n_seq);
+    const int64_t blocks64 = plan_blocks64(d->T, d->n_seq), blocks128 = plan_blocks128(d->T, d->n_seq);
     // the dQ kernel goes first: it leaves the row sums that the dK / dV kernel reads
-    const int rc = packed_launch<attn_packed_bwd_dq_kernel<D, CAUSAL>>("attn_packed_bwd_dq_kernel", blocks * d->H,
-                                                                       packed_lds_bytes(D, false), st, a);
-    if (rc) return rc;
-    return packed_launch<attn_packed_bwd_dkv_kernel<D, CAUSAL>>("attn_packed_bwd_dkv_kernel", blocks * d->Hkv,
-                                                                packed_lds_bytes(D, true), st, a);
+    const size_t lds = packed_lds_bytes(D);
+    if constexpr (D == 64) {
+        const int rc = packed_launch<attn_packed_bwd_dq_kernel<D, CAUSAL>>("attn_packed_bwd_dq_kernel", 256,
+                                                                           blocks64 * d->H, lds, st, a);
+        if (rc) return rc;
+        return packed_launch<attn_packed_bwd_dkv_kernel<CAUSAL>>("attn_packed_bwd_dkv_kernel", 256, blocks64 * d->Hkv,
+                                                                 attn_stages(D) * (2 * kTile * 2 + 512), st, a);
+    } else {
+        const int rc = packed_wide(d, d->H)
+                           ? packed_launch<attn_packed_bwd_dq128_kernel<D, CAUSAL>>("attn_packed_bwd_dq128_kernel", 256,
+                                                                                    blocks128 * d->H, lds, st, a)
+                           : packed_launch<attn_packed_bwd_dq_kernel<D, CAUSAL>>("attn_packed_bwd_dq_kernel", 256,
+                                                                                 blocks64 * d->H, lds, st, a);
+        if (rc) return rc;
+        // Whole backward, us, 64 | 128 keys per work-group: [32 query, 8 key / value heads] T = 2048: 203 | 303, 4096: 521 |
+        // 668, 16384 in 16 sequences: 919 | 841; [32, 32] T = 1024: 69.5 | 75.7, 2048: 173 | 161
+        if (packed_wide(d, d->Hkv))
+            return packed_launch<attn_packed_bwd_dkv8_kernel<D, CAUSAL, 2>>("attn_packed_bwd_dkv8_kernel", 512,
+                                                                            blocks128 * d->Hkv, dkv8_lds_bytes(D, 2), st, a);
+        return packed_launch<attn_packed_bwd_dkv8_kernel<D, CAUSAL, 1>>("attn_packed_bwd_dkv8_kernel", 512,
+                                                                        blocks64 * d->Hkv, dkv8_lds_bytes(D, 1), st, a);
+    }
 }
 
 }  // namespace pp

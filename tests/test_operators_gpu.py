@@ -153,6 +153,18 @@ def test_packed_attention_forward_and_backward(cut, H, Hkv, D, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,D", [(48, 48, 64), (48, 6, 64), (32, 32, 128), (32, 4, 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_attention_in_launches_that_fill_the_gpu(H, Hkv, D, causal):
+    """Sizes from which on the kernels take blocks of 128 rows (and, with as many key / value heads, of 128 keys)."""
+    cu = [0, 1, 130, 130, 386, 700, 1465, 1529, 2052]
+    b = Packed(cu, 2060, H, Hkv, D, seed=31)
+    b.qkv[cu[-1]:] = float("nan")
+    b.do[cu[-1]:] = float("nan")
+    b.run(causal).check(causal)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128])
 def test_packed_attention_with_large_scores_and_a_scale_of_the_callers(D):
     cu = [0, 100, 230]
