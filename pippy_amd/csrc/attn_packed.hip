@@ -23,6 +23,13 @@ constexpr int kPlanHeader = 4;   // int32: number of blocks of 64 rows, number o
 constexpr int kPlanBins = 2048;  // block indexes from here on count as one length class
 constexpr int kPlanThreads = 1024;
 
+// Chunk swizzle of a staged tile: row bits 1, 2, 3 reversed.  Rows start 32 of 64 banks apart.  A ds_read_b128 of one
+// chunk of 32 rows is served 16 lanes at a time, rows 0-3, 12-15, 20-27 and the rest: in either set the even rows, and
+// the odd ones, get eight different chunks.  A transposing read takes 32 lanes, 4 rows of 4 chunks aligned to 4: rows
+// two apart differ in the chunk's bit 2.  (Counted conflicts: SQ_LDS_BANK_CONFLICT 33 % of the active LDS cycles of
+// the forward with the swizzle of attn.hip.)
+__device__ __forceinline__ int swz_packed(int r) { return ((r & 2) << 1) | ((r & 4) >> 1) | ((r & 8) >> 3); }
+
 struct PackedArgs {
     const uint16_t* q; const uint16_t* k; const uint16_t* v;
     uint16_t* o; float* lse;
@@ -141,7 +148,7 @@ struct PackedTileLoader {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int row = (i * 4 + wave) * 8 + (lane >> 3);
-            voff[i] = row * (int)(stride_ * 2) + (((lane & 7) ^ swz_attn(row)) << 4);
+            voff[i] = row * (int)(stride_ * 2) + (((lane & 7) ^ swz_packed(row)) << 4);
         }
     }
     __device__ __forceinline__ void load(uint16_t* lds, int row0, int wave, int64_t extra = 0) const {
@@ -203,28 +210,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(c
     const float c = a.scale * kLog2e;
     const int partner = (lane ^ 32) << 2;
 
-    int stage = 0;
-    for (int j = 0; j < n_blocks; ++j) {
-        const int kt0 = j * 64 + 32 * half;
-        await_block<4 * DS, NS>(j, n_blocks);
-        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
-        const uint16_t* Ks = lds + stage * kStage;
+    // this wave's 32 keys of the block from key j * 64 on; MASKED: keys past the last visible one are left out
+    auto step = [&](auto masked_c, const uint16_t* Ks, int j) __attribute__((always_inline)) {
         const uint16_t* Vs = Ks + kOperand;
-        stage = stage + 1 == NS ? 0 : stage + 1;
-        if (kt0 >= w.len || (CAUSAL && kt0 > qw0 + 31)) continue;  // no key of this half is seen
         f32x16_t sacc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sacc[e] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8_t kf = read_row_frag(Ks + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t kf = read_row_frag<swz_packed>(Ks + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], sacc, 0, 0, 0);
         }
-        // sacc[v]: key kt0 + 8 (v / 4) + 4 lh + v % 4, query qi.  Keys past the last visible one are masked;
-        // wave-uniform: only the diagonal block and the end of the sequence pay for it.
-        const int last = CAUSAL ? (qr < w.len - 1 ? qr : w.len - 1) : w.len - 1;
-        if (kt0 + 31 > (CAUSAL ? qw0 : w.len - 1) || kt0 + 31 >= w.len) {
-            const int lim = last - kt0 - 4 * lh;
+        // sacc[v]: key 64 j + 32 half + 8 (v / 4) + 4 lh + v % 4, query qi
+        if constexpr (decltype(masked_c)::value) {
+            const int lim = (CAUSAL ? qr : w.len - 1) - j * 64 - 32 * half - 4 * lh;
 #pragma unroll
             for (int v = 0; v < 16; ++v)
                 if (8 * (v >> 2) + (v & 3) > lim) sacc[v] = -INFINITY;
@@ -260,10 +259,26 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(c
             const bf16x8_t pb = pack8(pv);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const bf16x8_t vf = read_col_frag(Vs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t vf = read_col_frag<swz_packed>(Vs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
                 oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, oacc[dt], 0, 0, 0);
             }
         }
+    };
+    // blocks that every query sees whole, without any masking code; then the diagonal or the end of the sequence
+    const int n_whole = CAUSAL ? w.j : w.len / 64;
+    int stage = 0, j = 0;
+    auto next = [&]() __attribute__((always_inline)) {
+        await_block<4 * DS, NS>(j, n_blocks);
+        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
+        const uint16_t* Ks = lds + stage * kStage;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        return Ks;
+    };
+    for (; j < n_whole; ++j) step(std::false_type{}, next(), j);
+    for (; j < n_blocks; ++j) {
+        const uint16_t* Ks = next();
+        const int kt0 = j * 64 + 32 * half;
+        if (kt0 < w.len && (!CAUSAL || kt0 <= qw0 + 31)) step(std::true_type{}, Ks, j);
     }
     l_run += __int_as_float(__builtin_amdgcn_ds_bpermute(partner, __float_as_int(l_run)));
 
@@ -360,7 +375,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd128_kerne
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int t = 0; t < N; ++t) {
-                const bf16x8_t kf = read_row_frag(Ks + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
+                const bf16x8_t kf = read_row_frag<swz_packed>(Ks + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], s[t], 0, 0, 0);
             }
         if constexpr (decltype(masked_c)::value) {
@@ -407,7 +422,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd128_kerne
                 const bf16x8_t pb = pack8(pv);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    const bf16x8_t vf = read_col_frag(Vs + (dt / 2) * kTile, kr + 32 * t + 16 * gp, 32 * (dt % 2), lane);
+                    const bf16x8_t vf = read_col_frag<swz_packed>(Vs + (dt / 2) * kTile, kr + 32 * t + 16 * gp, 32 * (dt % 2), lane);
                     oacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, oacc[dt], 0, 0, 0);
                 }
             }
@@ -518,15 +533,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
 #pragma unroll
         for (int e = 0; e < 16; ++e) dqacc[t][e] = 0.f;
 
-    int stage = 0;
-    for (int j = 0; j < n_blocks; ++j) {
-        const int kt0 = j * 64 + 32 * half;
-        await_block<4 * DS, NS>(j, n_blocks);
-        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
-        const uint16_t* Ks = lds + stage * kStage;
+    auto step = [&](auto masked_c, const uint16_t* Ks, int j) __attribute__((always_inline)) {
         const uint16_t* Vs = Ks + kOperand;
-        stage = stage + 1 == NS ? 0 : stage + 1;
-        if (kt0 >= w.len || (CAUSAL && kt0 > qw0 + 31)) continue;
         f32x16_t sacc, dpacc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -535,17 +543,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8_t kfr = read_row_frag(Ks + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
-            const bf16x8_t vfr = read_row_frag(Vs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t kfr = read_row_frag<swz_packed>(Ks + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t vfr = read_row_frag<swz_packed>(Vs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr, qf[ks], sacc, 0, 0, 0);
             dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr, dof[ks], dpacc, 0, 0, 0);
         }
         float dsv[16];
 #pragma unroll
         for (int v = 0; v < 16; ++v) dsv[v] = __builtin_amdgcn_exp2f(fmaf(sacc[v], c, -lse_q));
-        if ((CAUSAL && kt0 + 31 > qw0) || kt0 + 31 >= w.len) {
-            const int last = CAUSAL && qi < w.len - 1 ? qi : w.len - 1;
-            const int lim = last - kt0 - 4 * lh;
+        if constexpr (decltype(masked_c)::value) {
+            const int lim = (CAUSAL && qi < w.len - 1 ? qi : w.len - 1) - j * 64 - 32 * half - 4 * lh;
 #pragma unroll
             for (int v = 0; v < 16; ++v)
                 if (8 * (v >> 2) + (v & 3) > lim) dsv[v] = 0.f;
@@ -559,10 +566,25 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
             const bf16x8_t dsb = pack8(dsv + 8 * gp);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const bf16x8_t ktf = read_col_frag(Ks + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t ktf = read_col_frag<swz_packed>(Ks + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
                 dqacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktf, dsb, dqacc[dt], 0, 0, 0);
             }
         }
+    };
+    const int n_whole = CAUSAL ? w.j : w.len / 64;
+    int stage = 0, j = 0;
+    auto next = [&]() __attribute__((always_inline)) {
+        await_block<4 * DS, NS>(j, n_blocks);
+        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
+        const uint16_t* Ks = lds + stage * kStage;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        return Ks;
+    };
+    for (; j < n_whole; ++j) step(std::false_type{}, next(), j);
+    for (; j < n_blocks; ++j) {
+        const uint16_t* Ks = next();
+        const int kt0 = j * 64 + 32 * half;
+        if (kt0 < w.len && (!CAUSAL || kt0 <= qw0 + 31)) step(std::true_type{}, Ks, j);
     }
     d_sum += __shfl_xor(d_sum, 32, 64);
     // add the sums of the two halves: [grp][16 DT + 1 values][64 lanes] floats
@@ -654,8 +676,8 @@ __global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const Pac
         for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const bf16x8_t kfr = read_row_frag(Ks + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
-                const bf16x8_t vfr = read_row_frag(Vs + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
+                const bf16x8_t kfr = read_row_frag<swz_packed>(Ks + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
+                const bf16x8_t vfr = read_row_frag<swz_packed>(Vs + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr, qf[ks], s[t], 0, 0, 0);
                 dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr, dof[ks], dp[t], 0, 0, 0);
             }
@@ -681,7 +703,7 @@ __global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const Pac
                 const bf16x8_t dsb = pack8(ds);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    const bf16x8_t ktf = read_col_frag(Ks + (dt / 2) * kTile, kr + 32 * t + 16 * gp, 32 * (dt % 2), lane);
+                    const bf16x8_t ktf = read_col_frag<swz_packed>(Ks + (dt / 2) * kTile, kr + 32 * t + 16 * gp, 32 * (dt % 2), lane);
                     dqacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktf, dsb, dqacc[dt], 0, 0, 0);
                 }
             }
@@ -808,8 +830,8 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8_t qfr = read_row_frag(Qs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
-            const bf16x8_t ofr = read_row_frag(Os + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t qfr = read_row_frag<swz_packed>(Qs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t ofr = read_row_frag<swz_packed>(Os + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qfr, kf[ks], sacc, 0, 0, 0);
             dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ofr, vf[ks], dpacc, 0, 0, 0);
         }
@@ -843,8 +865,8 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
             const bf16x8_t dsb = pack8(dsv + 8 * gp);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const bf16x8_t otf = read_col_frag(Os + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
-                const bf16x8_t qtf = read_col_frag(Qs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t otf = read_col_frag<swz_packed>(Os + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t qtf = read_col_frag<swz_packed>(Qs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
                 dvacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(otf, pb, dvacc[dt], 0, 0, 0);
                 dkacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtf, dsb, dkacc[dt], 0, 0, 0);
             }
@@ -994,13 +1016,13 @@ __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const Pack
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8_t qfr = read_row_frag(Qs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t qfr = read_row_frag<swz_packed>(Qs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qfr, kf[ks], sacc, 0, 0, 0);
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8_t ofr = read_row_frag(Os + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
-            const bf16x8_t vfr = read_row_frag(Vs + (ks / 4) * kTile, vrow, 2 * (ks % 4) + lh);
+            const bf16x8_t ofr = read_row_frag<swz_packed>(Os + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
+            const bf16x8_t vfr = read_row_frag<swz_packed>(Vs + (ks / 4) * kTile, vrow, 2 * (ks % 4) + lh);
             dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ofr, vfr, dpacc, 0, 0, 0);
         }
         float pv[16], dsv[16];
@@ -1031,8 +1053,8 @@ __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const Pack
             const bf16x8_t dsb = pack8(dsv + 8 * gp);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const bf16x8_t otf = read_col_frag(Os + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
-                const bf16x8_t qtf = read_col_frag(Qs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t otf = read_col_frag<swz_packed>(Os + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
+                const bf16x8_t qtf = read_col_frag<swz_packed>(Qs + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
                 dvacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(otf, pb, dvacc[dt], 0, 0, 0);
                 dkacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qtf, dsb, dkacc[dt], 0, 0, 0);
             }

@@ -67,8 +67,9 @@ __device__ __forceinline__ void load_floats_to_lds(__amdgpu_buffer_rsrc_t rsrc, 
 }
 
 // Fragment with k along d: row `row` of the tile, 16-byte chunk `chunk`.
+template <int (*SWZ)(int) = swz_attn>
 __device__ __forceinline__ bf16x8_t read_row_frag(const uint16_t* tile, int row, int chunk) {
-    return *reinterpret_cast<const bf16x8_t*>(tile + row * 64 + ((chunk ^ swz_attn(row)) << 3));
+    return *reinterpret_cast<const bf16x8_t*>(tile + row * 64 + ((chunk ^ SWZ(row)) << 3));
 }
 
 // Fragment with k along the tile's rows, for 32 columns d0 .. d0+31 and the 16 rows r0 .. r0+15.
@@ -76,13 +77,14 @@ __device__ __forceinline__ bf16x8_t read_row_frag(const uint16_t* tile, int row,
 // in which a lane of a 32x32 MFMA result holds 8 of its 16 values, so that probabilities computed
 // in registers can be the other operand without a shuffle.  Inside each block of 16 lanes, lane
 // 4j + i fetches columns 4i .. 4i+3 of row j, and the hardware hands lane m the 4 rows of column m.
+template <int (*SWZ)(int) = swz_attn>
 __device__ __forceinline__ bf16x8_t read_col_frag(const uint16_t* tile, int r0, int d0, int lane) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const int g = lane >> 5, mb = (lane >> 4) & 1, j = (lane & 15) >> 2, i = lane & 3;
     const int d = d0 + 16 * mb + 4 * i;
     const int r_lo = r0 + 4 * g + j, r_hi = r_lo + 8;
-    const uint16_t* p_lo = tile + r_lo * 64 + (((d >> 3) ^ swz_attn(r_lo)) << 3) + (d & 7);
-    const uint16_t* p_hi = tile + r_hi * 64 + (((d >> 3) ^ swz_attn(r_hi)) << 3) + (d & 7);
+    const uint16_t* p_lo = tile + r_lo * 64 + (((d >> 3) ^ SWZ(r_lo)) << 3) + (d & 7);
+    const uint16_t* p_hi = tile + r_hi * 64 + (((d >> 3) ^ SWZ(r_hi)) << 3) + (d & 7);
     const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr_t)p_lo);
     const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr_t)p_hi);
     const s16x8_t v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
