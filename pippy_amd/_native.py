@@ -533,22 +533,27 @@ def moe_gate_bwd(dout, y, pos, topk_idx, gate, E: int, dlogits) -> None:
                                 dlogits.stride(0), T, Cc, current_stream()), "pp_moe_gate_bwd")
 
 
-def _moe_slots(who, topk_idx, t, T, name, dtype):
-    _need(t.dtype == dtype and t.is_contiguous() and t.shape == topk_idx.shape,
-          f"{who}: {name} must be contiguous {dtype} of topk_idx's shape")
+def _moe_slots(who, topk_idx, t, name):
+    if t.dtype != torch.float32 or t.shape != topk_idx.shape or not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be contiguous fp32 of topk_idx's shape")
 
 
 def _moe_logits(who, logits, topk_idx, scoring, E):
     """(rows, row stride, experts) of the logits."""
-    _need(logits.dim() == 2 and topk_idx.dim() == 2, f"{who}: logits [tokens, experts] and topk_idx [tokens, k]")
+    if logits.dim() != 2 or topk_idx.dim() != 2:
+        raise ValueError(f"{who}: logits [tokens, experts] and topk_idx [tokens, k]")
     T, cols = logits.shape
     ld, step = logits.stride()
-    E = cols if E is None else E
-    _need(step == 1 or cols == 1, f"{who}: the rows of logits must be contiguous")
-    _need(topk_idx.shape[0] == T and topk_idx.dtype == torch.int32 and topk_idx.is_contiguous(),
-          f"{who}: topk_idx must be contiguous int32 with a row per token")
-    _need(2 <= E <= cols, f"{who}: {E} experts in {cols} columns")
-    _need(scoring in MOE_SCORING, f"{who}: scoring {scoring!r}; known: {sorted(MOE_SCORING)}")
+    if E is None:
+        E = cols
+    if step != 1 and cols != 1:
+        raise ValueError(f"{who}: the rows of logits must be contiguous")
+    if topk_idx.dtype != torch.int32 or topk_idx.shape[0] != T or not topk_idx.is_contiguous():
+        raise ValueError(f"{who}: topk_idx must be contiguous int32 with a row per token")
+    if not 2 <= E <= cols:
+        raise ValueError(f"{who}: {E} experts in {cols} columns")
+    if scoring not in MOE_SCORING:
+        raise ValueError(f"{who}: scoring {scoring!r}; known: {sorted(MOE_SCORING)}")
     return T, ld if T > 1 else cols, E
 
 
@@ -559,10 +564,11 @@ def moe_route(logits, topk_idx, gate, *, bias=None, scoring: str = "softmax", n_
     ``logits`` carries padding columns after them; ``bias`` fp32 [E] enters the selection only."""
     stream = _stream_for(logits, topk_idx, gate, bias)
     T, ld, E = _moe_logits("moe_route", logits, topk_idx, scoring, E)
-    _moe_slots("moe_route", topk_idx, gate, T, "gate", torch.float32)
-    _need(bias is None or (bias.shape == (E,) and bias.dtype == torch.float32 and bias.is_contiguous()),
-          f"moe_route: bias must be contiguous fp32 [{E}]")
-    _need(group_score in MOE_GROUP_SCORE, f"moe_route: group_score {group_score!r}; known: {sorted(MOE_GROUP_SCORE)}")
+    _moe_slots("moe_route", topk_idx, gate, "gate")
+    if bias is not None and (bias.shape != (E,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+        raise ValueError(f"moe_route: bias must be contiguous fp32 [{E}]")
+    if group_score not in MOE_GROUP_SCORE:
+        raise ValueError(f"moe_route: group_score {group_score!r}; known: {sorted(MOE_GROUP_SCORE)}")
     d = MoeRouteDesc(logits.data_ptr(), ld, T, ptr(bias), topk_idx.data_ptr(), gate.data_ptr(), _pp_dtype(logits), E,
                      topk_idx.shape[1], MOE_SCORING[scoring], n_group, topk_group, MOE_GROUP_SCORE[group_score], renorm,
                      scale)
@@ -580,7 +586,7 @@ def moe_route_bwd(logits, topk_idx, dlogits, *, dgate=None, dout=None, y=None, p
           dlogits.stride(1) == 1, "moe_route_bwd: dlogits [tokens, at least the experts] of the type of logits")
     width = ld_dout = ld_y = 0
     if dgate is not None:
-        _moe_slots("moe_route_bwd", topk_idx, dgate, T, "dgate", torch.float32)
+        _moe_slots("moe_route_bwd", topk_idx, dgate, "dgate")
         dout = y = pos = None
     else:
         _need(dout is not None and y is not None and pos is not None,
@@ -959,8 +965,8 @@ def _packed_rows(name, t, shape):
 
 
 def _packed_stat(name, t, H, T):
-    _need(t.shape == (H, T) and t.dtype == torch.float32 and t.is_contiguous(),
-          f"packed attention: {name} must be contiguous fp32 {[H, T]}")
+    if t.shape != (H, T) or t.dtype != torch.float32 or not t.is_contiguous():
+        raise ValueError(f"packed attention: {name} must be contiguous fp32 {[H, T]}")
     return t.data_ptr()
 
 
@@ -968,7 +974,8 @@ def _packed_shapes(q, k, plan):
     _need(q.dim() == 3 and k.dim() == 3, "packed attention: q [rows, heads, D], k and v [rows, kv_heads, D]")
     T, H, D = q.shape
     Hkv = k.shape[1]
-    _need(plan.rows == T, f"packed attention: a plan of {plan.rows} rows for tensors of {T}")
+    if plan.rows != T:
+        raise ValueError(f"packed attention: a plan of {plan.rows} rows for tensors of {T}")
     return T, H, Hkv, D, (T, H, D), (T, Hkv, D)
 
 
