@@ -605,7 +605,8 @@ enum pp_op_kind {
     PP_OP_SWIGLU_FWD = 17, PP_OP_SWIGLU_BWD = 18, PP_OP_ROPE = 19, PP_OP_GEMM_SEG = 20,
     PP_OP_MOE_ROUTER = 21, PP_OP_MOE_PERMUTE = 22, PP_OP_MOE_GATHER = 23, PP_OP_MOE_COMBINE = 24,
     PP_OP_MOE_GATE_BWD = 25, PP_OP_GEMM_SWIGLU = 26, PP_OP_GEMM_DSWIGLU = 27, PP_OP_POSITION_IDS = 28,
-    PP_OP_GEMM_KSEG = 29, PP_OP_GEMM_SEG_KSEG = 30, PP_OP_GEMM_SEG_SWIGLU = 31, PP_OP_GEMM_SEG_DSWIGLU = 32
+    PP_OP_GEMM_KSEG = 29, PP_OP_GEMM_SEG_KSEG = 30, PP_OP_GEMM_SEG_SWIGLU = 31, PP_OP_GEMM_SEG_DSWIGLU = 32,
+    PP_OP_MOE_ROUTE = 33, PP_OP_MOE_ROUTE_BWD = 34, PP_OP_MOE_PERMUTE_WS = 35, PP_OP_DROPOUT = 36, PP_OP_RNG_ADVANCE = 37
 };
 
 /* Field use per kind (unused fields are ignored):
@@ -647,6 +648,14 @@ enum pp_op_kind {
  *                 device array of their seg_start arrays | i[7]: n_seg, i[8]: n_mb
  *   GEMM_SEG_SWIGLU  p: x w_gate_of w_up_of gu h seg_start | i: M N K ldx ldw ld_gu ldh n_seg
  *   GEMM_SEG_DSWIGLU p: dy w_down_t_of gu dgu seg_start | i: M N K ldy ldw ld_gu ld_dgu n_seg
+ *   MOE_ROUTE     p: logits bias topk_idx gate | i: ld T E topk n_group topk_group | f: scale
+ *                 | j: dtype scoring group_score renorm
+ *   MOE_ROUTE_BWD p: logits topk_idx dlogits dgate dout y pos | i: ld T E topk ld_dl cols_dl ld_dout ld_y C | f: scale
+ *                 | j: dtype scoring renorm
+ *   MOE_PERMUTE_WS p: expert_of_slot seg_start row_src pos workspace | i: n_slots E workspace_ints
+ *   DROPOUT       p: x resid y rng | i: ld_x ld_resid ld_y rows C | f: p | j: dtype site   (pp_dropout_add; a null resid
+ *                 is the backward, x = dy and y = dx)
+ *   RNG_ADVANCE   p: rng | i: step
  * flags bit 0 (PP_OP_SKIP): the op is stepped over.
  * flags bit 1 (PP_OP_GROUPED): a GEMM_BF16 op that may be launched together with the grouped
  * GEMM_BF16 ops next to it (they must not depend on each other); likewise consecutive grouped

@@ -27,7 +27,8 @@ EPI_DGELU_ERF, EPI_DGELU_TANH, EPI_ACCUM_F32, EPI_BIAS_RELU, EPI_DRELU, EPI_ACCU
  OP_ATTN_BWD, OP_EMBED_FWD, OP_EMBED_BWD, OP_CE_LOSS, OP_ACCUM_BF16, OP_ACCUM_F32, OP_COPY_ROWS,
  OP_FILL, OP_ACT_BWD, OP_SWIGLU_FWD, OP_SWIGLU_BWD, OP_ROPE, OP_GEMM_SEG, OP_MOE_ROUTER, OP_MOE_PERMUTE,
  OP_MOE_GATHER, OP_MOE_COMBINE, OP_MOE_GATE_BWD, OP_GEMM_SWIGLU, OP_GEMM_DSWIGLU, OP_POSITION_IDS,
- OP_GEMM_KSEG, OP_GEMM_SEG_KSEG, OP_GEMM_SEG_SWIGLU, OP_GEMM_SEG_DSWIGLU) = range(1, 33)
+ OP_GEMM_KSEG, OP_GEMM_SEG_KSEG, OP_GEMM_SEG_SWIGLU, OP_GEMM_SEG_DSWIGLU, OP_MOE_ROUTE, OP_MOE_ROUTE_BWD,
+ OP_MOE_PERMUTE_WS, OP_DROPOUT, OP_RNG_ADVANCE) = range(1, 38)
 SEG_ROWS, SEG_K = 0, 1
 OP_SKIP = 1
 OP_GROUPED = 2

@@ -480,6 +480,80 @@ def op_moe_gate_bwd(dout, y, pos, topk_idx, gate, E, dlogits) -> N.Op:
     return op
 
 
+def op_moe_route(logits, topk_idx, gate, E, *, bias=None, scoring="softmax", n_group=1, topk_group=1,
+                 group_score="max", renorm=True, scale=1.0) -> N.Op:
+    """``E``: number of experts (``logits`` may carry padding columns after them)."""
+    T, K = topk_idx.shape
+    assert logits.shape[0] == T and E <= logits.shape[1] and logits.stride(1) == 1
+    assert topk_idx.dtype == torch.int32 and topk_idx.is_contiguous()
+    assert gate.dtype == torch.float32 and gate.shape == (T, K) and gate.is_contiguous()
+    assert bias is None or (bias.dtype == torch.float32 and bias.numel() == E and bias.is_contiguous())
+    op = N.Op()
+    op.kind = N.OP_MOE_ROUTE
+    op.p[0], op.p[1], op.p[2], op.p[3] = logits.data_ptr(), _p(bias), topk_idx.data_ptr(), gate.data_ptr()
+    op.i[0], op.i[1], op.i[2], op.i[3], op.i[4], op.i[5] = logits.stride(0), T, E, K, n_group, topk_group
+    op.f[0] = scale
+    op.j[0], op.j[1], op.j[2], op.j[3] = (N._pp_dtype(logits), N.MOE_SCORING[scoring], N.MOE_GROUP_SCORE[group_score],
+                                          int(renorm))
+    return op
+
+
+def op_moe_route_bwd(logits, topk_idx, dlogits, E, dout, y, pos, *, scoring="softmax", renorm=True, scale=1.0) -> N.Op:
+    T, K = topk_idx.shape
+    assert logits.shape[0] == dlogits.shape[0] == dout.shape[0] == T and logits.dtype == dlogits.dtype
+    assert logits.stride(1) == 1 and dlogits.stride(1) == 1 and dout.stride(1) == 1 and y.stride(1) == 1
+    assert dout.shape[1] == y.shape[1] and pos.dtype == torch.int32 and pos.numel() == T * K
+    op = N.Op()
+    op.kind = N.OP_MOE_ROUTE_BWD
+    op.p[0], op.p[1], op.p[2] = logits.data_ptr(), topk_idx.data_ptr(), dlogits.data_ptr()
+    op.p[4], op.p[5], op.p[6] = dout.data_ptr(), y.data_ptr(), pos.data_ptr()
+    op.i[0], op.i[1], op.i[2], op.i[3] = logits.stride(0), T, E, K
+    op.i[4], op.i[5], op.i[6], op.i[7], op.i[8] = (dlogits.stride(0), dlogits.shape[1], dout.stride(0), y.stride(0),
+                                                   dout.shape[1])
+    op.f[0] = scale
+    op.j[0], op.j[1], op.j[2] = N._pp_dtype(logits), N.MOE_SCORING[scoring], int(renorm)
+    return op
+
+
+def op_moe_permute_ws(expert_of_slot, E, seg_start, row_src, pos, workspace) -> N.Op:
+    n = expert_of_slot.numel()
+    for t in (expert_of_slot, seg_start, row_src, pos, workspace):
+        assert t.dtype == torch.int32 and t.is_contiguous()
+    assert seg_start.numel() == E + 1 and row_src.numel() == n and pos.numel() == n
+    op = N.Op()
+    op.kind = N.OP_MOE_PERMUTE_WS
+    op.p[0], op.p[1], op.p[2], op.p[3], op.p[4] = (expert_of_slot.data_ptr(), seg_start.data_ptr(), row_src.data_ptr(),
+                                                   pos.data_ptr(), workspace.data_ptr())
+    op.i[0], op.i[1], op.i[2] = n, E, workspace.numel()
+    return op
+
+
+def op_dropout(x2d, y2d, rng, p: float, site: int, resid=None) -> N.Op:
+    """y = resid + mask * x / (1 - p); without ``resid`` also the backward (x: dy, y: dx)."""
+    assert x2d.shape == y2d.shape and x2d.dtype == y2d.dtype and x2d.stride(1) == 1 and y2d.stride(1) == 1
+    assert resid is None or (resid.shape == x2d.shape and resid.dtype == x2d.dtype and resid.stride(1) == 1)
+    op = N.Op()
+    op.kind = N.OP_DROPOUT
+    op.p[0], op.p[1], op.p[2], op.p[3] = x2d.data_ptr(), _p(resid), y2d.data_ptr(), rng.data_ptr()
+    if x2d.is_contiguous() and y2d.is_contiguous() and (resid is None or resid.is_contiguous()):
+        op.i[0] = op.i[1] = op.i[2] = op.i[4] = x2d.numel()
+        op.i[3] = 1
+    else:
+        op.i[0], op.i[1], op.i[2] = x2d.stride(0), resid.stride(0) if resid is not None else 0, y2d.stride(0)
+        op.i[3], op.i[4] = x2d.shape
+    op.f[0] = p
+    op.j[0], op.j[1] = N._pp_dtype(x2d), site
+    return op
+
+
+def op_rng_advance(rng, step: int = 1) -> N.Op:
+    op = N.Op()
+    op.kind = N.OP_RNG_ADVANCE
+    op.p[0] = rng.data_ptr()
+    op.i[0] = step
+    return op
+
+
 def op_ln_fwd(x, gamma, beta, y, mean, rstd, eps) -> N.Op:
     rows, Cc = x.shape
     assert x.is_contiguous() and y.is_contiguous() and y.shape == x.shape
@@ -714,6 +788,7 @@ class Builder:
         self._w_gemm: List[Tuple[N.Op, Optional[str]]] = []
         self._w_reduce: List[Tuple[N.Op, Optional[str]]] = []
         self._w_other: List[Tuple[N.Op, Optional[str]]] = []
+        self._n_dropouts = 0
         self.device = stage_prog.device
 
     # -- naming
@@ -760,6 +835,17 @@ class Builder:
     def scratch(self, name, shape, dtype) -> torch.Tensor:
         """Workspace valid inside one kernel sequence (never carried across passes)."""
         return self.sp.shared("scratch:" + name, shape, dtype, exact=False)
+
+    # -- dropout
+    def dropout_site(self) -> Tuple[torch.Tensor, int]:
+        """The {seed, offset} state of this microbatch slot and a site number of its own for one dropout.  The
+        state's offset advances once per forward pass, in front of its first dropout; the backward finds it as the
+        forward left it."""
+        rng = self.sp.rng_state(self.mb)
+        if self._n_dropouts == 0:
+            self.f(op_rng_advance(rng))
+        self._n_dropouts += 1
+        return rng, self._n_dropouts - 1
 
     # -- parameters
     def weight(self, p, padded=True):
@@ -844,7 +930,7 @@ _WRITTEN_FIELDS = {
     N.OP_ATTN_BWD: (6, 7, 8, 9), N.OP_ACT_BWD: (2,), N.OP_SWIGLU_BWD: (3, 4), N.OP_ROPE: (0,),
     N.OP_COPY_ROWS: (1,), N.OP_FILL: (0,), N.OP_ACCUM_BF16: (0,), N.OP_ACCUM_F32: (0,),
     N.OP_MOE_GATHER: (4,), N.OP_MOE_COMBINE: (4,), N.OP_MOE_GATE_BWD: (5,), N.OP_GEMM_DSWIGLU: (3,),
-    N.OP_GEMM_SEG_DSWIGLU: (3,),
+    N.OP_GEMM_SEG_DSWIGLU: (3,), N.OP_MOE_ROUTE_BWD: (2,), N.OP_DROPOUT: (2,),
     N.OP_EMBED_BWD: (2, 3), N.OP_CE_LOSS: (2, 3),
 }
 
@@ -932,8 +1018,12 @@ class StageProgram:
     """All microbatch programs of one stage plus its arenas and shared buffers."""
 
     def __init__(self, blocks: Sequence[nn.Module], module: nn.Module, device, training: bool,
-                 split_backward: bool, fused_accumulate: bool, is_first: bool, is_last: bool):
+                 split_backward: bool, fused_accumulate: bool, is_first: bool, is_last: bool,
+                 dropout_seed: int = 0):
         self.blocks = list(blocks)
+        self.dropout_seed = dropout_seed
+        self.dropout_mode: Tuple[bool, ...] = ()   # which blocks with dropout were in training mode when lowered
+        self._rng: Dict[int, torch.Tensor] = {}
         self.device = device
         self.training = training
         self.split_backward = split_backward
@@ -972,6 +1062,14 @@ class StageProgram:
             t = torch.empty(max(numel, 1), dtype=dtype, device=self.device)
             self._shared[full_key] = t
         return t[:numel].view(shape)
+
+    def rng_state(self, mb: int) -> torch.Tensor:
+        """int64 {seed, offset} of microbatch slot ``mb``: the slot in the upper half of the offset, the number of
+        forward passes so far in the lower.  It outlives the launch lists: a slot that is lowered again goes on."""
+        t = self._rng.get(mb)
+        if t is None:
+            t = self._rng[mb] = torch.tensor([self.dropout_seed, mb << 32], dtype=torch.int64, device=self.device)
+        return t
 
     def ones_f32(self, n: int) -> torch.Tensor:
         """A [1, n] row of ones (the left operand that turns an fp32 GEMM into a column sum)."""

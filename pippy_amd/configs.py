@@ -18,12 +18,12 @@ class DecoderLM(nn.Module):
     with tanh-GELU, final LayerNorm and an untied vocabulary projection."""
 
     def __init__(self, vocab=50257, max_seq=1024, dim=768, n_layers=12, n_heads=12, ffn=3072,
-                 dtype=torch.bfloat16, causal=True, pre_ln=True, activation="gelu_tanh", eps=1e-5):
+                 dtype=torch.bfloat16, causal=True, pre_ln=True, activation="gelu_tanh", eps=1e-5, dropout=0.0):
         super().__init__()
         self.embed = TokenEmbedding(vocab, max_seq, dim, dtype=dtype)
         self.h = nn.ModuleList([
             TransformerLayer(dim, n_heads, ffn, causal=causal, pre_ln=pre_ln, activation=activation,
-                             eps=eps, dtype=dtype) for _ in range(n_layers)])
+                             eps=eps, dtype=dtype, dropout=dropout) for _ in range(n_layers)])
         self.head = LMHead(dim, vocab, final_ln=pre_ln, eps=eps, dtype=dtype)
 
     def forward(self, ids):
@@ -86,15 +86,15 @@ def llama2_7b_stage(dtype=torch.bfloat16) -> LlamaStage:
 
 class MoEDecoderLM(nn.Module):
     """Mixtral-shaped decoder: token embedding (positions enter through the rotary embedding),
-    decoder layers whose feed-forward is a top-2 mixture of SwiGLU experts, final RMSNorm and an
-    untied vocabulary projection."""
+    decoder layers whose feed-forward is a top-2 mixture of SwiGLU experts (or one that routes as the
+    ``routing`` options of ``MoELayer`` say), final RMSNorm and an untied vocabulary projection."""
 
     def __init__(self, vocab=32000, dim=1024, n_layers=8, n_heads=16, ffn=4096, n_experts=8,
-                 dtype=torch.bfloat16, eps=1e-5, rope_theta=1e6):
+                 dtype=torch.bfloat16, eps=1e-5, rope_theta=1e6, **routing):
         super().__init__()
         self.embed = TokenEmbedding(vocab, 0, dim, dtype=dtype, positions=False)
         self.h = nn.ModuleList([
-            MoELayer(dim, n_heads, ffn, n_experts, eps=eps, rope_theta=rope_theta, dtype=dtype)
+            MoELayer(dim, n_heads, ffn, n_experts, eps=eps, rope_theta=rope_theta, dtype=dtype, **routing)
             for _ in range(n_layers)])
         self.head = LMHead(dim, vocab, final_ln="rms", eps=eps, dtype=dtype)
 

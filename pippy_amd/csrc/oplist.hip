@@ -203,6 +203,34 @@ static int run_one(const pp_op& op, pp_stream st) {
             return pp_moe_gate_bwd(op.p[0], op.i[0], op.p[1], op.i[1], static_cast<const int32_t*>(op.p[2]),
                                    static_cast<const int32_t*>(op.p[3]), static_cast<const float*>(op.p[4]),
                                    (int)op.i[2], (int)op.i[3], op.p[5], op.i[4], op.i[5], op.i[6], st);
+        case PP_OP_MOE_ROUTE: {
+            pp_moe_route_desc d = {};
+            d.logits = op.p[0]; d.bias = static_cast<const float*>(op.p[1]);
+            d.topk_idx = static_cast<int32_t*>(op.p[2]); d.gate = static_cast<float*>(op.p[3]);
+            d.ld = op.i[0]; d.T = op.i[1]; d.E = (int)op.i[2]; d.topk = (int)op.i[3];
+            d.n_group = (int)op.i[4]; d.topk_group = (int)op.i[5]; d.scale = op.f[0];
+            d.dtype = op.j[0]; d.scoring = op.j[1]; d.group_score = op.j[2]; d.renorm = op.j[3];
+            return pp_moe_route(&d, st);
+        }
+        case PP_OP_MOE_ROUTE_BWD: {
+            pp_moe_route_desc d = {};
+            d.logits = op.p[0]; d.topk_idx = static_cast<int32_t*>(op.p[1]); d.dlogits = op.p[2];
+            d.dgate = static_cast<const float*>(op.p[3]); d.dout = op.p[4]; d.y = op.p[5];
+            d.pos = static_cast<const int32_t*>(op.p[6]);
+            d.ld = op.i[0]; d.T = op.i[1]; d.E = (int)op.i[2]; d.topk = (int)op.i[3]; d.ld_dl = op.i[4];
+            d.cols_dl = (int)op.i[5]; d.ld_dout = op.i[6]; d.ld_y = op.i[7]; d.C = op.i[8]; d.scale = op.f[0];
+            d.dtype = op.j[0]; d.scoring = op.j[1]; d.renorm = op.j[2];
+            return pp_moe_route_bwd(&d, st);
+        }
+        case PP_OP_MOE_PERMUTE_WS:
+            return pp_moe_permute_ws(static_cast<const int32_t*>(op.p[0]), op.i[0], (int)op.i[1],
+                                     static_cast<int32_t*>(op.p[1]), static_cast<int32_t*>(op.p[2]),
+                                     static_cast<int32_t*>(op.p[3]), static_cast<int32_t*>(op.p[4]), op.i[2], st);
+        case PP_OP_DROPOUT:
+            return pp_dropout_add(op.p[0], op.i[0], op.p[1], op.i[1], op.p[2], op.i[2], op.i[3], op.i[4], op.j[0], op.f[0],
+                                  static_cast<const uint64_t*>(op.p[3]), (uint32_t)op.j[1], st);
+        case PP_OP_RNG_ADVANCE:
+            return pp_rng_advance(static_cast<uint64_t*>(op.p[0]), (uint64_t)op.i[0], st);
         default:
             return fail(PP_ERR_INVALID, "unknown op kind %d", op.kind);
     }
@@ -276,6 +304,8 @@ double op_work(const pp_op& op) {
             return 4.0 * (double)op.i[3] * (double)op.i[4];
         case PP_OP_MOE_COMBINE:  // read topk rows (+ the residual), write one, per token
             return 2.0 * ((double)op.i[1] + (op.p[3] ? 2.0 : 1.0)) * (double)op.i[4] * (double)op.i[5];
+        case PP_OP_DROPOUT:  // read x (and the residual), write y
+            return (op.p[1] ? 3.0 : 2.0) * (double)op.i[3] * (double)op.i[4] * (op.j[0] == PP_F32 ? 4.0 : 2.0);
         default:
             return 0.0;
     }

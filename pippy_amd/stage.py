@@ -126,6 +126,9 @@ class PipelineStageBase:
             m for m in submodule.modules()
             if (isinstance(m, nn.modules.dropout._DropoutNd) and m.p > 0)
             or (isinstance(m, nn.MultiheadAttention) and m.dropout > 0)]
+        # blocks with a dropout of their own, which runs inside the launch lists while they are in training mode
+        self._dropout_blocks = [blk for blk in self._blocks or ()
+                                if isinstance(getattr(blk, "dropout", None), float) and blk.dropout > 0]
         self._program: Optional[P.StageProgram] = None
         #: why this stage runs through torch autograd instead of HIP launch lists (None: it is native)
         self.eager_reason: Optional[str] = None
@@ -213,7 +216,8 @@ class PipelineStageBase:
                                            training=self.has_backward,
                                            split_backward=self.split_backward,
                                            fused_accumulate=self.fused_accumulate,
-                                           is_first=self.is_first, is_last=self.is_last)
+                                           is_first=self.is_first, is_last=self.is_last,
+                                           dropout_seed=self._dropout_seed())
             self._publish_grad_views()
         elif self._program.training != self.has_backward or \
                 self._program.split_backward != self.split_backward:
@@ -222,6 +226,20 @@ class PipelineStageBase:
             self._program.split_backward = self.split_backward
             self._program.mbs.clear()
         return self._program
+
+    def _follow_dropout_mode(self, sp: P.StageProgram) -> None:
+        """A launch list holds its dropouts or not: it is lowered again for the mode its blocks are in now."""
+        mode = tuple(blk.training for blk in self._dropout_blocks)
+        if mode != sp.dropout_mode:
+            if self.has_backward and self.fwd_cache:
+                raise RuntimeError(f"{self.log_prefix} was switched between training and eval mode with microbatches "
+                                   "in flight")
+            sp.dropout_mode = mode
+            sp.mbs.clear()
+
+    def _dropout_seed(self) -> int:
+        """Seed of this stage's dropout masks: torch's seed when the stage first runs, and the stage."""
+        return (torch.initial_seed() * 0x9E3779B97F4A7C15 + self.stage_index) % 2 ** 63
 
     def param_arena(self) -> "P.ParamArena":
         """The flat parameter / fp32-accumulator storage of a natively lowered stage (what the fused
@@ -350,6 +368,8 @@ class PipelineStageBase:
                 "before the stage is built (a stage built in training mode with p > 0 runs through torch "
                 "autograd), or set the dropout probabilities to 0")
         sp = self._stage_program()
+        if self._dropout_blocks:
+            self._follow_dropout_mode(sp)
         x, dx_target, patch = self._input_for(mb, args, kwargs)
         expected = self._exported_input_shape()
         if expected is not None and tuple(x.shape[1:]) != expected:

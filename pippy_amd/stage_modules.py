@@ -456,9 +456,13 @@ class TransformerLayer(NativeBlock):
     ``attn.c_proj``, ``ln_2``, ``mlp.c_fc``, ``mlp.c_proj``) with ``nn.Linear`` weights [out, in]."""
 
     def __init__(self, dim: int, n_heads: int, ffn: int, *, causal: bool = True, pre_ln: bool = True,
-                 activation: str = "gelu_tanh", eps: float = 1e-5, dtype=torch.bfloat16, init_std=0.02):
+                 activation: str = "gelu_tanh", eps: float = 1e-5, dtype=torch.bfloat16, init_std=0.02,
+                 dropout: float = 0.0):
         super().__init__()
         assert dim % n_heads == 0 and activation in ("gelu_tanh", "gelu_erf", "relu")
+        if not 0.0 <= dropout < 1.0:
+            raise ValueError(f"dropout must lie in [0, 1), not {dropout}")
+        self.dropout = float(dropout)
         self.dim, self.n_heads, self.ffn = dim, n_heads, ffn
         self.causal, self.pre_ln, self.activation = causal, pre_ln, activation
         self.ln_1 = nn.LayerNorm(dim, eps=eps, dtype=dtype)
@@ -473,6 +477,7 @@ class TransformerLayer(NativeBlock):
             nn.init.normal_(lin.weight, std=init_std)
             nn.init.zeros_(lin.bias)
 
+    dropout = 0.0          # rate of the dropouts on the two residual branches, in training mode
     attn_scale = None      # the factor on the attention scores; None: 1 / sqrt(head size)
     n_kv_heads = None      # fewer key / value heads than query heads (multi-query: 1); None: as many
 
@@ -487,12 +492,34 @@ class TransformerLayer(NativeBlock):
         o = F.scaled_dot_product_attention(q, k, v, is_causal=self.causal, scale=self.attn_scale)
         return self.attn.c_proj(o.transpose(1, 2).reshape(Bn, S, Cc))
 
+    def _drop(self, branch, which):
+        """Dropout of residual branch ``which`` (0: attention, 1: feed-forward).  The launch lists draw their masks
+        from their own counter-based generator: the same distribution, other masks than torch's."""
+        return F.dropout(branch, self.dropout, self.training) if self.dropout > 0 else branch
+
     def forward(self, x):
         if self.pre_ln:
-            x = x + self._attention(self.ln_1(x))
-            return x + self.mlp.c_proj(_torch_act(self.mlp.c_fc(self.ln_2(x)), self.activation))
-        x = self.ln_1(x + self._attention(x))
-        return self.ln_2(x + self.mlp.c_proj(_torch_act(self.mlp.c_fc(x), self.activation)))
+            x = x + self._drop(self._attention(self.ln_1(x)), 0)
+            return x + self._drop(self.mlp.c_proj(_torch_act(self.mlp.c_fc(self.ln_2(x)), self.activation)), 1)
+        x = self.ln_1(x + self._drop(self._attention(x), 0))
+        return self.ln_2(x + self._drop(self.mlp.c_proj(_torch_act(self.mlp.c_fc(x), self.activation)), 1))
+
+    def _lower_branch(self, b, name, lin, h2d, resid):
+        """Emits resid + dropout(lin(h)); returns it and the emitter of the branch's output gradient, dy -> d lin(h)."""
+        if not (self.dropout > 0 and self.training):
+            y, _ = lower_linear(b, name, lin, h2d, epilogue=N.EPI_BIAS_RESIDUAL, aux_in=resid)
+            return y, lambda dy2d: dy2d
+        rng, site = b.dropout_site()
+        branch, _ = lower_linear(b, name + ".branch", lin, h2d)
+        y = b.act(name, tuple(branch.shape))
+        b.f(P.op_dropout(branch, y, rng, self.dropout, site, resid=resid))
+
+        def backward(dy2d):
+            d_branch = b.grad(name + ".d_branch", tuple(branch.shape))
+            b.i(P.op_dropout(dy2d, d_branch, rng, self.dropout, site))
+            return d_branch
+
+        return y, backward
 
     # the q|k|v projection: one fused layer here; subclasses around a user's model may hold three
     def _qkv_layers(self):
@@ -540,23 +567,24 @@ class TransformerLayer(NativeBlock):
         ln1, mean1, rstd1 = lower_layernorm(b, "ln1", self.ln_1, x2d)
         qkv = self._lower_qkv(b, ln1)
         att, attention_backward = lower_attention(b, qkv, Bn, S, H, self.causal, n_kv_heads=self.n_kv_heads, scale=self.attn_scale)
-        x2, _ = lower_linear(b, "x2", self.attn.c_proj, att, epilogue=N.EPI_BIAS_RESIDUAL, aux_in=x2d)
+        x2, attention_branch = self._lower_branch(b, "x2", self.attn.c_proj, att, x2d)
         ln2, mean2, rstd2 = lower_layernorm(b, "ln2", self.ln_2, x2)
         # (the derivative of a ReLU is read off its output; a GELU's needs the value before it)
         h, h_pre = lower_linear(b, "h", self.mlp.c_fc, ln2, epilogue=act,
                                 save_pre=b.training and self.activation != "relu")
         if self.activation == "relu":
             h_pre = h
-        y, _ = lower_linear(b, "y", self.mlp.c_proj, h, epilogue=N.EPI_BIAS_RESIDUAL, aux_in=x2)
+        y, feed_forward_branch = self._lower_branch(b, "y", self.mlp.c_proj, h, x2)
 
         def bwd(dy, need_dx, dx_out):
             dy2d = dy.view(T, Cc)
             # feed-forward: dI through c_proj carries gelu'(h_pre) in its epilogue
-            d_hpre = linear_backward(b, "c_proj", self.mlp.c_proj, h, dy2d, dx_epilogue=dact, dx_aux=h_pre)
+            d_hpre = linear_backward(b, "c_proj", self.mlp.c_proj, h, feed_forward_branch(dy2d), dx_epilogue=dact,
+                                     dx_aux=h_pre)
             d_ln2 = linear_backward(b, "c_fc", self.mlp.c_fc, ln2, d_hpre)
             d_x2 = layernorm_backward(b, "ln2", self.ln_2, x2, mean2, rstd2, d_ln2, dres=dy2d)
             # attention
-            d_att = linear_backward(b, "attn_proj", self.attn.c_proj, att, d_x2)
+            d_att = linear_backward(b, "attn_proj", self.attn.c_proj, att, attention_branch(d_x2))
             dqkv = attention_backward(d_att)
             d_ln1 = self._qkv_backward(b, ln1, dqkv)
             dx = layernorm_backward(b, "ln1", self.ln_1, x2d, mean1, rstd1, d_ln1, dres=d_x2,
@@ -573,24 +601,25 @@ class TransformerLayer(NativeBlock):
         act, dact = _ACT_EPI[self.activation], _ACT_DEPI[self.activation]
         qkv = self._lower_qkv(b, x2d)
         att, attention_backward = lower_attention(b, qkv, Bn, S, H, self.causal, n_kv_heads=self.n_kv_heads, scale=self.attn_scale)
-        a, _ = lower_linear(b, "a", self.attn.c_proj, att, epilogue=N.EPI_BIAS_RESIDUAL, aux_in=x2d)
+        a, attention_branch = self._lower_branch(b, "a", self.attn.c_proj, att, x2d)
         x1, mean1, rstd1 = lower_layernorm(b, "ln1", self.ln_1, a)
         h, h_pre = lower_linear(b, "h", self.mlp.c_fc, x1, epilogue=act,
                                 save_pre=b.training and self.activation != "relu")
         if self.activation == "relu":
             h_pre = h
-        f, _ = lower_linear(b, "f", self.mlp.c_proj, h, epilogue=N.EPI_BIAS_RESIDUAL, aux_in=x1)
+        f, feed_forward_branch = self._lower_branch(b, "f", self.mlp.c_proj, h, x1)
         y, mean2, rstd2 = lower_layernorm(b, "ln2", self.ln_2, f)
 
         def bwd(dy, need_dx, dx_out):
             # a sum of two gradients in front of a LayerNorm is formed by the residual epilogue
             # (without a bias) of the input-gradient GEMM that produces one of them
             d_f = layernorm_backward(b, "ln2", self.ln_2, f, mean2, rstd2, dy.view(T, Cc))
-            d_hpre = linear_backward(b, "c_proj", self.mlp.c_proj, h, d_f, dx_epilogue=dact, dx_aux=h_pre)
+            d_hpre = linear_backward(b, "c_proj", self.mlp.c_proj, h, feed_forward_branch(d_f), dx_epilogue=dact,
+                                     dx_aux=h_pre)
             d_x1 = linear_backward(b, "c_fc", self.mlp.c_fc, x1, d_hpre, dx_epilogue=N.EPI_BIAS_RESIDUAL,
                                    dx_aux=d_f)
             d_a = layernorm_backward(b, "ln1", self.ln_1, a, mean1, rstd1, d_x1)
-            d_att = linear_backward(b, "attn_proj", self.attn.c_proj, att, d_a)
+            d_att = linear_backward(b, "attn_proj", self.attn.c_proj, att, attention_branch(d_a))
             dqkv = attention_backward(d_att)
             dx = self._qkv_backward(b, x2d, dqkv, dx_epilogue=N.EPI_BIAS_RESIDUAL, dx_aux=d_a,
                                     dx_out=dx_out.view(T, Cc) if dx_out is not None else None)
@@ -964,10 +993,11 @@ class _ExpertTensors:
 class _MoEFeedForward:
     """The sparse feed-forward half of a Mixtral-style layer (mixed into a Llama-style layer class):
     a softmax router picks two of ``n_experts`` SwiGLU experts per token, weights renormalised over the
-    pair.  Needs ``self.n_experts``, ``self.ffn``, ``self._experts`` (an expert-weight bank),
+    pair, or routes as ``self.routing`` says.  Needs ``self.n_experts``, ``self.ffn``, ``self._experts`` (an expert-weight bank),
     ``self._router`` (an ``nn.Linear``-shaped layer) and ``self.forced_routing``."""
 
     TOPK = 2
+    routing = None     # dict of pp_moe_route's options (without the bias) when the router is not the top-2 softmax
     _pp_batch_weight_grads = True      # see PipelineStageBase.prefers_batched_weight_grads
 
     def _padded_experts(self) -> int:
@@ -979,19 +1009,41 @@ class _MoEFeedForward:
     def _feed_forward(self, h):
         shape = h.shape
         h = h.reshape(-1, shape[-1])
-        probs = torch.softmax(self._router(h).float(), dim=-1)
+        logits = self._router(h).float()
+        how = self.routing or {}
+        probs = torch.softmax(logits, dim=-1) if how.get("scoring", "softmax") == "softmax" else torch.sigmoid(logits)
         if self.forced_routing:
             idx = self.forced_routing.pop(0).to(h.device)
-        else:
+        elif self.routing is None:
             idx = torch.sort(probs, dim=-1, descending=True, stable=True).indices[:, :2]
+        else:
+            idx = self._select(logits, probs)
         top = probs.gather(-1, idx)
-        gate = top / top.sum(-1, keepdim=True)
+        gate = top / top.sum(-1, keepdim=True) if how.get("renorm", True) else top
+        gate = gate * how.get("scale", 1.0)
         y = torch.zeros(h.shape, dtype=torch.float32, device=h.device)
         for e in range(self.n_experts):
             tok, slot = torch.where(idx == e)
             if tok.numel():
                 y = y.index_add(0, tok, gate[tok, slot, None] * self._experts.apply(e, h[tok]).float())
         return y.to(h.dtype).reshape(shape)
+
+    def _balance_bias(self):
+        return None
+
+    def _select(self, logits, probs):
+        """Torch statement of the selection (see ``pp_moe_route``)."""
+        how, bias = self.routing, self._balance_bias()
+        choice = probs if bias is None else probs + bias.to(probs)
+        rank = logits if bias is None else choice
+        if how["n_group"] > 1:
+            by_group = (choice if how["group_score"] == "top2" else rank).unflatten(-1, (how["n_group"], -1))
+            value = by_group.topk(min(2, by_group.shape[-1]), -1).values.sum(-1) if how["group_score"] == "top2" \
+                else by_group.amax(-1)
+            kept = torch.sort(value, dim=-1, descending=True, stable=True).indices[:, :how["topk_group"]]
+            shut = torch.ones_like(value, dtype=torch.bool).scatter(1, kept, False)
+            rank = rank.unflatten(-1, (how["n_group"], -1)).masked_fill(shut[..., None], float("-inf")).flatten(-2)
+        return torch.sort(rank, dim=-1, descending=True, stable=True).indices[:, :self.TOPK]
 
     def _pointer_list(self, b, name, tensors):
         t = b.sp.shared(f"moe_ptrs:{id(self)}:{name}", (len(tensors),), torch.int64)
@@ -1011,11 +1063,19 @@ class _MoEFeedForward:
         lower_linear(b, "router", router, n2, out=logits)
         idx = b.act("topk_idx", (T, K), torch.int32)
         gate = b.act("gate", (T, K), torch.float32)
-        b.f(P.op_moe_router(logits, idx, gate, E))
+        how = self.routing
+        if how is None:
+            b.f(P.op_moe_router(logits, idx, gate, E))
+        else:
+            b.f(P.op_moe_route(logits, idx, gate, E, bias=self._balance_bias_on(b.device), **how))
         seg = b.act("seg_start", (E + 1,), torch.int32)
         row_src = b.act("row_src", (R,), torch.int32)
         pos = b.act("pos", (R,), torch.int32)
-        b.f(P.op_moe_permute(idx.view(-1), E, seg, row_src, pos))
+        if how is None:
+            b.f(P.op_moe_permute(idx.view(-1), E, seg, row_src, pos))
+        else:
+            ws = b.scratch("moe_permute", (N.moe_permute_workspace(R, E),), torch.int32)
+            b.f(P.op_moe_permute_ws(idx.view(-1), E, seg, row_src, pos, ws))
         xp = b.act("xp", (R, Cc))
         b.f(P.op_moe_gather(n2, row_src, K, xp))
 
@@ -1050,7 +1110,11 @@ class _MoEFeedForward:
             d_yp = b.grad("d_yp", (R, Cc))
             b.i(P.op_moe_gather(dy2d, row_src, K, d_yp, scale=gate.view(-1)))
             dlogits = b.grad("dlogits", (T, Ep))
-            b.i(P.op_moe_gate_bwd(dy2d, yp, pos, idx, gate, E, dlogits))
+            if how is None:
+                b.i(P.op_moe_gate_bwd(dy2d, yp, pos, idx, gate, E, dlogits))
+            else:
+                b.i(P.op_moe_route_bwd(logits, idx, dlogits, E, dy2d, yp, pos, scoring=how["scoring"],
+                                       renorm=how["renorm"], scale=how["scale"]))
             w2t, ld2t = pointers("w2t", bank.transposed(b, "down"))
             if fused:
                 dgu = b.grad("dgu", (R, 2 * ffn))
@@ -1100,23 +1164,56 @@ class MoELayer(_MoEFeedForward, LlamaLayer):
     ``block_sparse_moe.experts.<e>.w1 / w2 / w3``.  The launch-list form takes 2 .. 64 experts (a count
     that is not a multiple of 8 runs with the router weight and the logits padded to one).
 
+    Any other router (up to 512 experts, 16 per token): ``top_k``; ``scoring`` "softmax" or "sigmoid"; ``n_group`` /
+    ``topk_group`` / ``group_score`` ("max", "top2") keep the experts of the best groups only; ``norm_topk`` renormalises
+    the weights; ``routed_scale`` multiplies them; ``balance_bias=True`` adds the fp32 buffer
+    ``block_sparse_moe.balance_bias`` [n_experts] to the scores for the selection (no gradient: a training loop updates
+    it in place from the expert loads).  See ``pp_moe_route``.
+
     ``forced_routing`` (a list of int64 [tokens, 2] tensors, one per forward call, consumed in
     order) overrides the expert selection of the torch statement; a comparison against a lower
     precision run uses it so that tokens whose second and third logits nearly tie do not count as
     errors of the arithmetic."""
 
     def __init__(self, dim: int, n_heads: int, ffn: int, n_experts: int = 8, *, eps: float = 1e-5,
-                 rope_theta: float = 1e6, dtype=torch.bfloat16, init_std=0.02, n_kv_heads: Optional[int] = None):
+                 rope_theta: float = 1e6, dtype=torch.bfloat16, init_std=0.02, n_kv_heads: Optional[int] = None,
+                 top_k: int = 2, scoring: str = "softmax", n_group: int = 1, topk_group: int = 1,
+                 group_score: str = "max", norm_topk: bool = True, routed_scale: float = 1.0,
+                 balance_bias: bool = False):
         LlamaLayer.__init__(self, dim, n_heads, ffn, eps=eps, rope_theta=rope_theta, dtype=dtype,
                             init_std=init_std, n_kv_heads=n_kv_heads)
         del self.mlp
-        assert 2 <= n_experts <= 64
+        if (top_k, scoring, n_group, norm_topk, routed_scale, balance_bias) != (2, "softmax", 1, True, 1.0, False) or \
+                n_experts > 64:
+            if scoring not in N.MOE_SCORING or group_score not in N.MOE_GROUP_SCORE:
+                raise ValueError(f"scoring {scoring!r}, group_score {group_score!r}; known: {sorted(N.MOE_SCORING)}, "
+                                 f"{sorted(N.MOE_GROUP_SCORE)}")
+            if not 2 <= n_experts <= 512 or n_group < 1 or n_experts % n_group or not 1 <= topk_group <= n_group or \
+                    not 1 <= top_k <= min(16, n_experts // n_group * topk_group):
+                raise ValueError(f"{top_k} of {n_experts} experts in {topk_group} of {n_group} groups: 2 to 512 experts, at "
+                                 "most 16 per token, out of groups that hold as many")
+            self.TOPK = top_k
+            self.routing = dict(scoring=scoring, n_group=n_group, topk_group=topk_group, group_score=group_score,
+                                renorm=norm_topk, scale=routed_scale)
+        assert 2 <= n_experts <= 512
         self.n_experts = n_experts
         self.block_sparse_moe = nn.Module()
         self.block_sparse_moe.gate = nn.Linear(dim, n_experts, bias=False, dtype=dtype)
         nn.init.normal_(self.block_sparse_moe.gate.weight, std=init_std)
         self.block_sparse_moe.experts = nn.ModuleList([_Expert(dim, ffn, dtype, init_std) for _ in range(n_experts)])
+        if balance_bias:
+            self.block_sparse_moe.register_buffer("balance_bias", torch.zeros(n_experts))
         self.forced_routing = None
+
+    def _balance_bias(self):
+        return getattr(self.block_sparse_moe, "balance_bias", None)
+
+    def _balance_bias_on(self, device):
+        """The bias where the launch lists read it: the module's own buffer, fp32 on the device."""
+        bias = self._balance_bias()
+        if bias is not None and (bias.device != device or bias.dtype != torch.float32):
+            bias = self.block_sparse_moe.balance_bias = bias.to(device=device, dtype=torch.float32)
+        return bias
 
     @property
     def _router(self):
