@@ -646,37 +646,23 @@ __global__ __launch_bounds__(kPermThreads) void moe_permute_place_kernel(const i
                                                                          int32_t* __restrict__ pos) {
     __shared__ int cnt[kPermWaves][kPermMaxE];
     __shared__ int wave_total[kPermWaves];
-    __shared__ int share[2][kPermThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int e[kPermRounds], r[kPermRounds];
     perm_rank(cnt, ids, n, E, bits, e, r);
-    // expert tid: its total over all work-groups, and what lies in front of this one.  All threads share the loads:
-    // with E experts, 1024 / E sets of them (E rounded up to a power of two) take every so manyth work-group.
+    // expert tid: its total over all work-groups, and what lies in front of this one
     int total = 0, before = 0;
-    if (gridDim.x == 1) {
-        if (tid < E) {
+    if (tid < E) {
+        if (gridDim.x == 1) {
 #pragma unroll
             for (int w = 0; w < kPermWaves; ++w) total += cnt[w][tid];
-        }
-    } else {
-        const int e_of = tid & ((1 << bits) - 1), set = tid >> bits, sets = kPermThreads >> bits;
-        if (e_of < E) {
-#pragma unroll 8
-            for (unsigned b = set; b < gridDim.x; b += sets) {
-                const int v = ws[(int64_t)b * E + e_of];
+        } else {
+#pragma unroll 16
+            for (unsigned b = 0; b < gridDim.x; ++b) {
+                const int v = ws[(int64_t)b * E + tid];
                 total += v;
                 before += b < blockIdx.x ? v : 0;
             }
         }
-        share[0][tid] = total;
-        share[1][tid] = before;
-        __syncthreads();
-        total = before = 0;
-        if (tid < E)
-            for (int q = 0; q < sets; ++q) {
-                total += share[0][tid + (q << bits)];
-                before += share[1][tid + (q << bits)];
-            }
     }
     int upto = total;  // running sum over the experts: inside the wave, then over the waves
 #pragma unroll
