@@ -385,7 +385,7 @@ typedef struct pp_moe_route_desc {
 int pp_moe_route(const pp_moe_route_desc* desc, pp_stream stream);
 int pp_moe_route_bwd(const pp_moe_route_desc* desc, pp_stream stream);
 
-/* pp_moe_permute for up to 1024 experts and many slots: the same outputs bit for bit, on as many work-groups as
+/* pp_moe_permute for up to 1024 experts and many slots (at most 2^24): the same outputs bit for bit, on as many work-groups as
  * the slots fill.  workspace: pp_moe_permute_workspace_ints(n_slots, E) int32, not shared by calls that may
  * overlap; that function returns -1 for sizes out of range.  (index_add_ / sort of the torch form of the block,
  * pippy/_PipelineStage.py:420-428.) */

@@ -579,17 +579,18 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
 }
 
 // ---- permutation --------------------------------------------------------------------------------
-// A stable counting sort by expert.  A work-group takes kPermSlots consecutive slots, a wave a consecutive part of
+// A stable counting sort by expert.  A work-group takes 1024 ROUNDS consecutive slots, a wave a consecutive part of
 // them, 64 at a time: one ballot per bit of the expert index gives every lane the set of lanes that hold its
 // expert; its rank is the wave's count so far plus the members in front of it, and the first member counts for all.
-// Up to kPermSlots slots are one launch.  More are two: the counts of every work-group, then every work-group
-// adds up the counts of all and of those in front of it and places its slots.
-// 16 waves of 256 slots: twice as many work-groups of half the size double the counts that each one reads.
+// Up to 4096 slots are one launch of one work-group.  More are two: the counts of every work-group, then every
+// work-group adds up the counts of all and of those in front of it and places its slots.  More rounds mean fewer
+// work-groups and fewer counts to read but longer chains; us for 1, 2, 4, 8 rounds, 256 experts: 32768 slots 8.0,
+// 8.8, 14.1, 20.3; 262144: 15.1, 12.8, 14.5, 20.9; 1048576: 68, 30, 23, 26; 4194304: 918, 262, 99, 74.
 constexpr int kPermMaxE = 1024;
 constexpr int kPermThreads = 1024;
 constexpr int kPermWaves = kPermThreads / 64;
-constexpr int kPermRounds = 4;
-constexpr int kPermSlots = kPermThreads * kPermRounds;
+constexpr int kPermOneLaunch = 4 * kPermThreads;
+constexpr int64_t kPermMaxSlots = 1 << 24;
 
 __device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
     unsigned long long m = __ballot(e >= 0);
@@ -602,19 +603,20 @@ __device__ __forceinline__ unsigned long long same_expert(int e, int bits) {
 
 // Ranks this work-group's slots inside their wave: e[q] the expert of the lane's q-th slot (-1: none), r[q] its rank;
 // cnt[wave][E] the wave's counts.
+template <int ROUNDS>
 __device__ __forceinline__ void perm_rank(int (*cnt)[kPermMaxE], const int32_t* ids, int64_t n, int E, int bits,
-                                          int (&e)[kPermRounds], int (&r)[kPermRounds]) {
+                                          int (&e)[ROUNDS], int (&r)[ROUNDS]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t first = (int64_t)blockIdx.x * kPermSlots + wave * (64 * kPermRounds) + lane;
+    const int64_t first = (int64_t)blockIdx.x * (ROUNDS * kPermThreads) + wave * (64 * ROUNDS) + lane;
 #pragma unroll
-    for (int q = 0; q < kPermRounds; ++q) {
+    for (int q = 0; q < ROUNDS; ++q) {
         e[q] = first + q * 64 < n ? ids[first + q * 64] : -1;
         if (e[q] >= E) e[q] = -1;
     }
     for (int i = lane; i < E; i += 64) cnt[wave][i] = 0;
     wave_lds_fence();
 #pragma unroll
-    for (int q = 0; q < kPermRounds; ++q) {
+    for (int q = 0; q < ROUNDS; ++q) {
         const unsigned long long m = same_expert(e[q], bits);
         r[q] = 0;
         if (e[q] >= 0) r[q] = cnt[wave][e[q]] + __popcll(m & ((1ull << lane) - 1ull));
@@ -626,10 +628,11 @@ __device__ __forceinline__ void perm_rank(int (*cnt)[kPermMaxE], const int32_t* 
     __syncthreads();
 }
 
+template <int ROUNDS>
 __global__ __launch_bounds__(kPermThreads) void moe_permute_count_kernel(const int32_t* __restrict__ ids, int64_t n,
                                                                          int E, int bits, int32_t* __restrict__ ws) {
     __shared__ int cnt[kPermWaves][kPermMaxE];
-    int e[kPermRounds], r[kPermRounds];
+    int e[ROUNDS], r[ROUNDS];
     perm_rank(cnt, ids, n, E, bits, e, r);
     if ((int)threadIdx.x < E) {
         int s = 0;
@@ -639,6 +642,7 @@ __global__ __launch_bounds__(kPermThreads) void moe_permute_count_kernel(const i
     }
 }
 
+template <int ROUNDS>
 __global__ __launch_bounds__(kPermThreads) void moe_permute_place_kernel(const int32_t* __restrict__ ids, int64_t n,
                                                                          int E, int bits, const int32_t* __restrict__ ws,
                                                                          int32_t* __restrict__ seg_start,
@@ -647,7 +651,7 @@ __global__ __launch_bounds__(kPermThreads) void moe_permute_place_kernel(const i
     __shared__ int cnt[kPermWaves][kPermMaxE];
     __shared__ int wave_total[kPermWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int e[kPermRounds], r[kPermRounds];
+    int e[ROUNDS], r[ROUNDS];
     perm_rank(cnt, ids, n, E, bits, e, r);
     // expert tid: its total over all work-groups, and what lies in front of this one
     int total = 0, before = 0;
@@ -688,9 +692,9 @@ __global__ __launch_bounds__(kPermThreads) void moe_permute_place_kernel(const i
         }
     }
     __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * kPermSlots + wave * (64 * kPermRounds) + lane;
+    const int64_t first = (int64_t)blockIdx.x * (ROUNDS * kPermThreads) + wave * (64 * ROUNDS) + lane;
 #pragma unroll
-    for (int q = 0; q < kPermRounds; ++q) {
+    for (int q = 0; q < ROUNDS; ++q) {
         const int64_t i = first + q * 64;
         if (i >= n) continue;
         const int at = e[q] >= 0 ? cnt[wave][e[q]] + r[q] : -1;
@@ -699,7 +703,31 @@ __global__ __launch_bounds__(kPermThreads) void moe_permute_place_kernel(const i
     }
 }
 
-static int64_t perm_groups(int64_t n) { return n > 0 ? (n + kPermSlots - 1) / kPermSlots : 1; }
+// At most 64 R work-groups of R rounds (8: any number of them).
+static int perm_rounds(int64_t n) {
+    if (n <= kPermOneLaunch) return 4;
+    return n <= 64 * 1024 ? 1 : n <= 4 * 64 * 1024 ? 2 : n <= 16 * 64 * 1024 ? 4 : 8;
+}
+static int64_t perm_groups(int64_t n) {
+    const int64_t slots = (int64_t)perm_rounds(n) * kPermThreads;
+    return n > 0 ? (n + slots - 1) / slots : 1;
+}
+
+template <int ROUNDS>
+static int perm_launch(const int32_t* ids, int64_t n, int E, int32_t* seg_start, int32_t* row_src, int32_t* pos,
+                       int32_t* ws, hipStream_t st) {
+    int bits = 0;
+    while ((1 << bits) < E) ++bits;
+    const dim3 grid((unsigned)perm_groups(n));
+    if (grid.x > 1) {
+        hipLaunchKernelGGL(moe_permute_count_kernel<ROUNDS>, grid, dim3(kPermThreads), 0, st, ids, n, E, bits, ws);
+        const int rc = check_launch("moe_permute_count_kernel");
+        if (rc) return rc;
+    }
+    hipLaunchKernelGGL(moe_permute_place_kernel<ROUNDS>, grid, dim3(kPermThreads), 0, st, ids, n, E, bits, ws, seg_start,
+                       row_src, pos);
+    return check_launch("moe_permute_place_kernel");
+}
 
 template <typename LT, bool SIGMOID, bool BIASED>
 static int route_launch(const RouteArgs& a, hipStream_t st) {
@@ -800,7 +828,7 @@ extern "C" int pp_moe_route_bwd(const pp_moe_route_desc* d, pp_stream stream) {
 }
 
 extern "C" int64_t pp_moe_permute_workspace_ints(int64_t n_slots, int E) {
-    if (n_slots < 0 || n_slots > 0x7fffffff || E < 1 || E > kPermMaxE) return -1;
+    if (n_slots < 0 || n_slots > kPermMaxSlots || E < 1 || E > kPermMaxE) return -1;
     return perm_groups(n_slots) * E;
 }
 
@@ -809,21 +837,16 @@ extern "C" int pp_moe_permute_ws(const int32_t* expert_of_slot, int64_t n_slots,
                                  pp_stream stream) {
     const int64_t need = pp_moe_permute_workspace_ints(n_slots, E);
     if (need < 0 || !seg_start || (n_slots > 0 && (!expert_of_slot || !row_src || !pos)))
-        return fail(PP_ERR_INVALID, "pp_moe_permute_ws: bad arguments (n_slots=%lld E=%d, at most %d experts)",
-                    (long long)n_slots, E, kPermMaxE);
+        return fail(PP_ERR_INVALID, "pp_moe_permute_ws: bad arguments (n_slots=%lld E=%d, at most %d experts and %lld slots)",
+                    (long long)n_slots, E, kPermMaxE, (long long)kPermMaxSlots);
     if (!workspace || workspace_ints < need)
         return fail(PP_ERR_INVALID, "pp_moe_permute_ws: workspace of %lld ints, needs %lld", (long long)workspace_ints,
                     (long long)need);
-    int bits = 0;
-    while ((1 << bits) < E) ++bits;
-    const dim3 grid((unsigned)perm_groups(n_slots));
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (grid.x > 1) {
-        hipLaunchKernelGGL(moe_permute_count_kernel, grid, dim3(kPermThreads), 0, st, expert_of_slot, n_slots, E, bits, workspace);
-        const int rc = check_launch("moe_permute_count_kernel");
-        if (rc) return rc;
+    switch (perm_rounds(n_slots)) {
+        case 1: return perm_launch<1>(expert_of_slot, n_slots, E, seg_start, row_src, pos, workspace, st);
+        case 2: return perm_launch<2>(expert_of_slot, n_slots, E, seg_start, row_src, pos, workspace, st);
+        case 4: return perm_launch<4>(expert_of_slot, n_slots, E, seg_start, row_src, pos, workspace, st);
+        default: return perm_launch<8>(expert_of_slot, n_slots, E, seg_start, row_src, pos, workspace, st);
     }
-    hipLaunchKernelGGL(moe_permute_place_kernel, grid, dim3(kPermThreads), 0, st, expert_of_slot, n_slots, E, bits, workspace,
-                       seg_start, row_src, pos);
-    return check_launch("moe_permute_place_kernel");
 }

@@ -511,7 +511,7 @@ def test_routing_tells_choices_apart_that_differ_by_less_than_a_rounding():
 # ---- permutation ------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,E", [(0, 4), (1, 1), (10, 64), (96, 64), (2048, 8), (2049, 3), (5001, 256), (40000, 1024),
-                                 (70001, 129)])
+                                 (70001, 129), (262145, 17), (1048577, 300)])
 def test_permutation_of_many_slots_bit_exact(n, E):
     N = native()
     g = torch.Generator().manual_seed(n)

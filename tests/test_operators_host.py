@@ -159,7 +159,7 @@ def test_routing_backward_refuses(change, match):
 def test_permutation_refuses():
     L = N.lib()
     assert L.pp_moe_permute_workspace_ints(10, 1025) == L.pp_moe_permute_workspace_ints(-1, 8) == \
-        L.pp_moe_permute_workspace_ints(10, 0) == L.pp_moe_permute_workspace_ints(2 ** 31, 8) == -1
+        L.pp_moe_permute_workspace_ints(10, 0) == L.pp_moe_permute_workspace_ints(2 ** 24 + 1, 8) == -1
     need = L.pp_moe_permute_workspace_ints(5000, 100)
     assert need >= 100
     refused(L.pp_moe_permute_ws(A, 5000, 1025, A, A, A, A, 1 << 20, None), "at most 1024 experts")
