@@ -1077,7 +1077,9 @@ class _MoEFeedForward:
             ws = b.scratch("moe_permute", (N.moe_permute_workspace(R, E),), torch.int32)
             b.f(P.op_moe_permute_ws(idx.view(-1), E, seg, row_src, pos, ws))
         xp = b.act("xp", (R, Cc))
-        b.f(P.op_moe_gather(n2, row_src, K, xp))
+        # a router that leaves a token fewer experts than slots (logits of -infinity) places fewer rows
+        n_rows = None if how is None else seg[E:]
+        b.f(P.op_moe_gather(n2, row_src, K, xp, n_rows=n_rows))
 
         def pointers(name, pair):
             tensors, ld = pair
@@ -1108,7 +1110,7 @@ class _MoEFeedForward:
         def backward(dy2d):
             # expert rows receive the output gradient of their token times the routing weight
             d_yp = b.grad("d_yp", (R, Cc))
-            b.i(P.op_moe_gather(dy2d, row_src, K, d_yp, scale=gate.view(-1)))
+            b.i(P.op_moe_gather(dy2d, row_src, K, d_yp, scale=gate.view(-1), n_rows=n_rows))
             dlogits = b.grad("dlogits", (T, Ep))
             if how is None:
                 b.i(P.op_moe_gate_bwd(dy2d, yp, pos, idx, gate, E, dlogits))

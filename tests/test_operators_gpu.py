@@ -665,6 +665,57 @@ def test_operators_refuse_tensors_that_do_not_fit():
             call()
 
 
+@pytest.mark.gpu
+def test_launch_lists_hold_the_operators():
+    """Route, permute, gather, dropout and the router's gradient as launch-list ops, with tokens that go to no expert."""
+    from pippy_amd import _program as P
+    N = native()
+    g = torch.Generator().manual_seed(2)
+    T, E, K, C = 60, 20, 3, 64
+    logits = torch.randn(T, 24, generator=g).to(torch.bfloat16)
+    logits[7:20, :E] = float("-inf")
+    logits[20:25, 2:E] = float("-inf")
+    ld = logits.to(DEV)
+    x = torch.randn(T, C, generator=g).to(torch.bfloat16).to(DEV)
+    rng, seed, offset = rng_state(seed=3, offset=10)
+    idx, gate = torch.empty(T, K, dtype=torch.int32, device=DEV), torch.empty(T, K, device=DEV)
+    seg = torch.empty(E + 1, dtype=torch.int32, device=DEV)
+    row_src = torch.full((T * K,), 2 ** 30, dtype=torch.int32, device=DEV)      # never read past the placed rows
+    pos = torch.empty(T * K, dtype=torch.int32, device=DEV)
+    ws = torch.empty(N.moe_permute_workspace(T * K, E), dtype=torch.int32, device=DEV)
+    rows = torch.full((T * K, C), SENTINEL, dtype=torch.bfloat16, device=DEV)
+    y, dx, wide = torch.empty_like(x), torch.empty_like(x), torch.empty(T, 2 * C, dtype=torch.bfloat16, device=DEV)
+    dl = torch.full_like(ld, 9.0)
+    how = dict(scoring="sigmoid", n_group=4, topk_group=2, group_score="top2")
+    ops = P.OpList()
+    ops.append(P.op_rng_advance(rng))
+    ops.append(P.op_moe_route(ld, idx, gate, E, **how))
+    ops.append(P.op_moe_permute_ws(idx.view(-1), E, seg, row_src, pos, ws))
+    ops.append(P.op_moe_gather(x, row_src, K, rows, n_rows=seg[E:]))
+    ops.append(P.op_moe_combine(rows, pos, K, y, gate=gate.view(-1)))
+    ops.append(P.op_dropout(y, wide[:, C:], rng, 0.4, 5, resid=x))
+    ops.append(P.op_dropout(x, dx, rng, 0.4, 5))
+    ops.append(P.op_moe_route_bwd(ld, idx, dl, E, x, rows, pos, scoring="sigmoid"))
+    ops.run()
+    torch.cuda.synchronize()
+    assert rng.tolist() == [seed, offset + 1]
+    ref_idx, ref_gate = O.moe_route(logits[:, :E].double(), K, **how)
+    assert torch.equal(idx.cpu().long(), ref_idx)
+    placed = int((ref_idx >= 0).sum())
+    assert int(seg[E]) == placed < T * K and bool((rows[placed:] == SENTINEL).all())
+    # every placed row is its token's, so the weighted sum is the token times the sum of its weights
+    total = gate.cpu().double().sum(-1, keepdim=True)
+    want = x.cpu().double() * total
+    within(y, want, (U + 2.0 ** -20) * want.abs(), "combine")
+    f = O.dropout_factors(T * C, 0.4, seed, offset + 1, 5).view(T, C)
+    want = x.cpu().double() + f * y.cpu().double()
+    within(wide[:, C:], want, 2.0 ** -22 * (1 + want.abs()) + U * want.abs(), "dropout")
+    within(dx, f * x.cpu().double(), (U + 2.0 ** -22) * (f * x.cpu().double()).abs(), "dx")
+    # the rows of a token are all alike: the gradient of renormalised weights is zero but for roundings of |x|^2
+    size = x.cpu().double().pow(2).sum(-1, keepdim=True)
+    assert bool((dl.cpu().double().abs() <= 2.0 ** -16 * size * (ref_idx >= 0).any(-1, keepdim=True)).all())
+
+
 # ---- together ---------------------------------------------------------------------------------------
 @pytest.mark.gpu
 def test_a_step_of_all_of_them_as_a_layer_uses_them():
