@@ -353,7 +353,8 @@ int pp_moe_gate_bwd(const void* dout, int64_t ld_dout, const void* y, int64_t ld
  *   gate[t, k] = scale * s[idx_k] / (renorm ? sum_j s[idx_j] : 1)         (a sum of 0 gives gates of 0)
  * A logit of -infinity takes its expert out: it is not selected and counts in no sum; a token with fewer than
  * topk experts left has topk_idx -1 and gate 0 in its last slots, which the permutations drop (position -1).  A
- * NaN logit makes the token's softmax weights NaN and ranks behind every number.
+ * NaN logit ranks behind every number; it makes the token's softmax weights NaN (renormalised ones only if it is
+ * selected, since they are formed from the selected logits alone).
  * Backward: the gradient of the logits from dgate (fp32 [T, topk]), or, with dgate null, from
  * dgate[t, k] = <dout[t, :], y[pos[t, k], :]> formed on the way (dout bf16 [T, C], y the bf16 expert rows, pos as
  * pp_moe_permute gives it; a negative position or index counts as no contribution).  The bias gets no gradient.
@@ -528,8 +529,9 @@ int pp_attn_bwd(const pp_attn_desc* desc, pp_stream stream);
  * A non-finite value row reaches, besides the queries that see it, earlier queries of its block of rows (0 * NaN
  * inside a matrix product), never another sequence.
  *
- * The plan says which blocks of rows there are, longest first.  pp_attn_packed_plan builds it on the device from
- * cu_seqlens (one small launch, no host synchronisation); every layer and both directions of a batch share it.
+ * The plan says which blocks of rows there are, the dearest first.  pp_attn_packed_plan builds it on the device from
+ * cu_seqlens (one small launch, no host synchronisation); every layer and both directions of a batch share it.  The
+ * grids are sized by T and n_seq: a sequence that is empty costs a few work-groups that end at once.
  * plan: int32 [pp_attn_packed_plan_ints(n_seq, T)], 16-byte aligned; n_seq and T of a call must be the plan's.
  * ---------------------------------------------------------------------------------------- */
 typedef struct pp_attn_packed_desc {

@@ -11,15 +11,14 @@
 // are per-lane scalars and the probabilities sit in registers as the second product wants its operand.
 //
 // Which work-group takes which block is a plan built on the device once per batch (pp_attn_packed_plan) and
-// shared by all layers and both directions: the blocks of all sequences, the latest blocks first.  Under a
-// causal mask block j of a sequence costs j + 1 steps, so a launch begins with its longest work-groups and
-// fills up with ever shorter ones, however unequal the sequences are.
+// shared by all layers and both directions: the blocks of all sequences, the dearest first, so that a launch begins
+// with its longest work-groups and fills up with ever shorter ones, however unequal the sequences are.
 #include "attn_tile.h"
 #include <math.h>
 
 namespace pp {
 
-constexpr int kPlanHeader = 4;   // int32: number of blocks of 64 rows, number of blocks of 128 rows, 0, 0
+constexpr int kPlanHeader = 4;   // int32: number of entries of each of the four lists
 constexpr int kPlanBins = 2048;  // block indexes from here on count as one length class
 constexpr int kPlanThreads = 1024;
 
@@ -40,7 +39,7 @@ struct PackedArgs {
     int64_t T;
     int32_t H, G;       // query heads; query heads per key / value head
     const int32_t* plan;
-    int32_t cap64;      // entries that the plan reserves for blocks of 64 rows
+    int32_t cap64, cap128;  // entries that the plan reserves for blocks of 64 and of 128 rows
     float scale;
 };
 
@@ -48,9 +47,11 @@ __host__ __device__ inline int64_t plan_blocks64(int64_t T, int64_t n_seq) { ret
 __host__ __device__ inline int64_t plan_blocks128(int64_t T, int64_t n_seq) { return T / 128 + n_seq; }
 
 // ---- the plan -----------------------------------------------------------------------------------
-// One work-group; a wave takes a sequence at a time, its lanes the blocks.  Counting sort by block index, the
-// highest first; the order inside a class is left to the atomics, since it only says which work-group does
-// what.  Entries: {first row of the sequence, its length, block index, 0}.
+// Four lists, one work-group each: blocks of 64 and of 128 rows, in the order for a causal mask and in the order
+// without one.  Entries {first row of the sequence, its length, block index, 0}, dearest blocks first: under a causal
+// mask a block costs as many steps as its index says, without one as its sequence has blocks.  A counting sort over
+// that; a wave takes a sequence at a time, its lanes the blocks.  The order inside a class is left to the atomics,
+// since it only says which work-group does what.
 __global__ __launch_bounds__(kPlanThreads) void attn_packed_plan_kernel(const int32_t* __restrict__ cu, int n_seq,
                                                                         int T, int32_t* __restrict__ plan,
                                                                         int cap64, int cap128) {
@@ -58,46 +59,42 @@ __global__ __launch_bounds__(kPlanThreads) void attn_packed_plan_kernel(const in
     __shared__ int part[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     constexpr int kWaves = kPlanThreads / 64;
-    int4* entries = reinterpret_cast<int4*>(plan + kPlanHeader);
-    for (int pass = 0; pass < 2; ++pass) {
-        const int block = pass == 0 ? 64 : 128;
-        const int cap = pass == 0 ? cap64 : cap128;
-        for (int i = tid; i < kPlanBins; i += kPlanThreads) cursor[i] = 0;
+    const bool wide = blockIdx.x & 1, full = blockIdx.x >> 1;
+    const int block = wide ? 128 : 64, cap = wide ? cap128 : cap64;
+    int4* entries = reinterpret_cast<int4*>(plan + kPlanHeader) + (full ? cap64 + cap128 : 0) + (wide ? cap64 : 0);
+    for (int i = tid; i < kPlanBins; i += kPlanThreads) cursor[i] = 0;
+    __syncthreads();
+    for (int place = 0; place < 2; ++place) {
+        for (int b = wave; b < n_seq; b += kWaves) {
+            // bounds that are out of order or out of range make an empty sequence
+            const int r0 = cu[b], r1 = cu[b + 1];
+            const int len = (r0 >= 0 && r1 > r0 && r1 <= T) ? r1 - r0 : 0;
+            const int nb = len / block + (len % block != 0);
+            for (int j = lane; j < nb; j += 64) {
+                const int cost = full ? nb - 1 : j;
+                const int at = atomicAdd(&cursor[cost < kPlanBins - 1 ? cost : kPlanBins - 1], 1);
+                if (place && (uint32_t)at < (uint32_t)cap) entries[at] = make_int4(r0, len, j, 0);
+            }
+        }
         __syncthreads();
-        for (int place = 0; place < 2; ++place) {
-            for (int b = wave; b < n_seq; b += kWaves) {
-                // bounds that are out of order or out of range make an empty sequence
-                const int r0 = cu[b], r1 = cu[b + 1];
-                const int len = (r0 >= 0 && r1 > r0 && r1 <= T) ? r1 - r0 : 0;
-                const int nb = len / block + (len % block != 0);
-                for (int j = lane; j < nb; j += 64) {
-                    const int bin = j < kPlanBins - 1 ? j : kPlanBins - 1;
-                    const int at = atomicAdd(&cursor[bin], 1);
-                    if (place && at < cap) entries[at] = make_int4(r0, len, j, 0);
-                }
-            }
+        if (place) break;
+        // counts -> first places: a class begins behind all dearer ones (two classes per thread)
+        const int hi = kPlanBins - 1 - 2 * tid, lo = hi - 1;
+        const int n_hi = cursor[hi], n_lo = cursor[lo];
+        part[tid] = n_hi + n_lo;
+        __syncthreads();
+        for (int o = 1; o < kPlanThreads; o <<= 1) {
+            const int add = tid >= o ? part[tid - o] : 0;
             __syncthreads();
-            if (place) break;
-            // counts -> first places: a class begins behind all higher ones (two classes per thread)
-            const int hi = kPlanBins - 1 - 2 * tid, lo = hi - 1;
-            const int n_hi = cursor[hi], n_lo = cursor[lo];
-            part[tid] = n_hi + n_lo;
-            __syncthreads();
-            for (int o = 1; o < kPlanThreads; o <<= 1) {
-                const int add = tid >= o ? part[tid - o] : 0;
-                __syncthreads();
-                part[tid] += add;
-                __syncthreads();
-            }
-            const int begin = part[tid] - n_hi - n_lo;
-            cursor[hi] = begin;
-            cursor[lo] = begin + n_hi;
-            if (tid == kPlanThreads - 1) plan[pass] = part[tid] < cap ? part[tid] : cap;
+            part[tid] += add;
             __syncthreads();
         }
-        entries += cap64;
+        const int begin = part[tid] - n_hi - n_lo;
+        cursor[hi] = begin;
+        cursor[lo] = begin + n_hi;
+        if (tid == kPlanThreads - 1) plan[blockIdx.x] = (uint32_t)part[tid] < (uint32_t)cap ? part[tid] : cap;
+        __syncthreads();
     }
-    if (tid < 2) plan[2 + tid] = 0;
 }
 static_assert(kPlanBins == 2 * kPlanThreads, "the scan takes two classes per thread");
 
@@ -111,8 +108,11 @@ struct PackedBlock {
 // With a multiple of 8 heads every XCD takes its own heads (keys and values of a head in one L2; the heads of a
 // group that shares them are neighbours), longest block of all its heads first.  Otherwise the blocks are dealt
 // out in order: consecutive work-groups go to different XCDs, and every XCD gets an equal share of each length.
-__device__ __forceinline__ bool packed_block_of(const PackedArgs& a, int heads, const int4* entries, int n_blocks,
-                                                PackedBlock* w) {
+template <bool CAUSAL, bool WIDE>
+__device__ __forceinline__ bool packed_block_of(const PackedArgs& a, int heads, PackedBlock* w) {
+    const int4* entries = reinterpret_cast<const int4*>(a.plan + kPlanHeader) + (CAUSAL ? 0 : a.cap64 + a.cap128) +
+                          (WIDE ? a.cap64 : 0);
+    const int n_blocks = a.plan[(CAUSAL ? 0 : 2) + (WIDE ? 1 : 0)];
     const uint32_t bid = blockIdx.x;
     uint32_t t, h;
     if (heads % 8 == 0) {
@@ -129,8 +129,8 @@ __device__ __forceinline__ bool packed_block_of(const PackedArgs& a, int heads, 
     w->len = __builtin_amdgcn_readfirstlane(e.y);
     w->j = __builtin_amdgcn_readfirstlane(e.z);
     w->h = (int)h;
-    // a plan made for more rows than this call has
-    return w->row0 >= 0 && w->len > 0 && w->row0 + w->len <= a.T;
+    // a plan that was not made for this call: nothing outside the tensors is touched
+    return w->row0 >= 0 && w->row0 + w->len <= a.T && w->j >= 0 && (int64_t)w->j * (WIDE ? 128 : 64) < w->len;
 }
 
 // Loader of 64-row blocks of a sequence.  Every block gets a resource of its own that begins at the block (so
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(c
     const int grp = wave & 1, half = wave >> 1;
     const int l32 = lane & 31, lh = lane >> 5;
     PackedBlock w;
-    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader), a.plan[0], &w)) return;
+    if (!packed_block_of<CAUSAL, false>(a, a.H, &w)) return;
     const int q0 = w.j * 64, qw0 = q0 + 32 * grp, qi = qw0 + l32;
     const int hk = w.h / a.G;
 
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd128_kerne
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, lh = lane >> 5;
     PackedBlock w;
-    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader) + a.cap64, a.plan[1], &w)) return;
+    if (!packed_block_of<CAUSAL, true>(a, a.H, &w)) return;
     const int q0 = w.j * 128, qw0 = q0 + 32 * wave, qi = qw0 + l32;
     const int hk = w.h / a.G;
 
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
     const int grp = wave & 1, half = wave >> 1;
     const int l32 = lane & 31, lh = lane >> 5;
     PackedBlock w;
-    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader), a.plan[0], &w)) return;
+    if (!packed_block_of<CAUSAL, false>(a, a.H, &w)) return;
     const int q0 = w.j * 64, qw0 = q0 + 32 * grp, qi = qw0 + l32;
     const int hk = w.h / a.G;
 
@@ -626,7 +626,7 @@ __global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const Pac
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, lh = lane >> 5;
     PackedBlock w;
-    if (!packed_block_of(a, a.H, reinterpret_cast<const int4*>(a.plan + kPlanHeader) + a.cap64, a.plan[1], &w)) return;
+    if (!packed_block_of<CAUSAL, true>(a, a.H, &w)) return;
     const int q0 = w.j * 128, qw0 = q0 + 32 * wave, qi = qw0 + l32;
     const int hk = w.h / a.G;
 
@@ -761,7 +761,7 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
     const int grp = wave & 1, half = wave >> 1;
     const int l32 = lane & 31, lh = lane >> 5;
     PackedBlock w;  // w.h: key / value head
-    if (!packed_block_of(a, a.H / a.G, reinterpret_cast<const int4*>(a.plan + kPlanHeader), a.plan[0], &w)) return;
+    if (!packed_block_of<CAUSAL, false>(a, a.H / a.G, &w)) return;
     const int nbq = (w.len + 63) / 64;
     // the plan's order is by query work; a key block sees the most queries where a query block sees the fewest
     // keys, so the block index counts from the end here
@@ -942,9 +942,7 @@ __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const Pack
     const int set = wave >> 2, lwave = wave & 3;          // waves 0-3 load Q, waves 4-7 dO
     const int l32 = lane & 31, lh = lane >> 5;
     PackedBlock w;  // w.h: key / value head
-    if (!packed_block_of(a, a.H / a.G, reinterpret_cast<const int4*>(a.plan + kPlanHeader) + (KB == 2 ? a.cap64 : 0),
-                         a.plan[KB - 1], &w))
-        return;
+    if (!packed_block_of<CAUSAL, KB == 2>(a, a.H / a.G, &w)) return;
     // the plan's order is by query work; under a causal mask key blocks count from the end (see above)
     const int jk = CAUSAL ? (w.len + 64 * KB - 1) / (64 * KB) - 1 - w.j : w.j;
     const int kv0 = jk * (64 * KB), kvi = kv0 + 32 * grp + l32;
@@ -1123,8 +1121,7 @@ static_assert(dkv8_lds_bytes(128, 1) <= 160 * 1024 && dkv8_lds_bytes(128, 2) <= 
 // ---- entry points -------------------------------------------------------------------------------
 static int packed_check(const char* who, const pp_attn_packed_desc* d, bool bwd) {
     if (!d) return fail(PP_ERR_INVALID, "%s: null descriptor", who);
-    if (d->T < 0 || d->T > 0x7fffffc0ll || d->n_seq < 0 || d->n_seq > 0x7fffffc0ll || d->H <= 0 || d->Hkv <= 0 ||
-        d->H % d->Hkv)
+    if (pp_attn_packed_plan_ints(d->n_seq, d->T) < 0 || d->H <= 0 || d->H > (1 << 17) || d->Hkv <= 0 || d->H % d->Hkv)
         return fail(PP_ERR_INVALID, "%s: bad shape (T=%lld n_seq=%lld H=%lld Hkv=%lld)", who, (long long)d->T,
                     (long long)d->n_seq, (long long)d->H, (long long)d->Hkv);
     if (d->D != 64 && d->D != 128)
@@ -1164,6 +1161,7 @@ static PackedArgs packed_args(const pp_attn_packed_desc* d) {
     a.G = (int32_t)(d->H / d->Hkv);
     a.plan = d->plan;
     a.cap64 = (int32_t)plan_blocks64(d->T, d->n_seq);
+    a.cap128 = (int32_t)plan_blocks128(d->T, d->n_seq);
     a.scale = d->scale;
     return a;
 }
@@ -1243,15 +1241,16 @@ using namespace pp;
 
 extern "C" int64_t pp_attn_packed_plan_ints(int64_t n_seq, int64_t T) {
     if (n_seq < 0 || T < 0 || n_seq > 0x7fffffc0ll || T > 0x7fffffc0ll) return -1;
-    return kPlanHeader + 4 * (plan_blocks64(T, n_seq) + plan_blocks128(T, n_seq));
+    const int64_t entries = 2 * (plan_blocks64(T, n_seq) + plan_blocks128(T, n_seq));
+    return entries > 0x7fffffffll ? -1 : kPlanHeader + 4 * entries;
 }
 
 extern "C" int pp_attn_packed_plan(const int32_t* cu_seqlens, int64_t n_seq, int64_t T, int32_t* plan, pp_stream stream) {
-    if (pp_attn_packed_plan_ints(n_seq, T) < 0 || plan_blocks64(T, n_seq) > 0x7fffffc0ll)
+    if (pp_attn_packed_plan_ints(n_seq, T) < 0)
         return fail(PP_ERR_INVALID, "pp_attn_packed_plan: bad shape (n_seq=%lld T=%lld)", (long long)n_seq, (long long)T);
     if (!plan || !aligned(plan, 16) || (n_seq > 0 && !cu_seqlens))
         return fail(PP_ERR_INVALID, "pp_attn_packed_plan: null pointer, or a plan that is not 16-byte aligned");
-    hipLaunchKernelGGL(attn_packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream),
+    hipLaunchKernelGGL(attn_packed_plan_kernel, dim3(4), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream),
                        cu_seqlens, (int)n_seq, (int)T, plan, (int)plan_blocks64(T, n_seq), (int)plan_blocks128(T, n_seq));
     return check_launch("attn_packed_plan_kernel");
 }
