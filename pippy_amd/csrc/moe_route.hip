@@ -18,6 +18,7 @@ namespace pp {
 constexpr int kRouteMaxE = 512;
 constexpr int kRouteMaxK = 16;
 constexpr int kRouteMaxGroups = 64;
+constexpr int kRouteList = 64;  // entries of the list that the experts are selected from
 
 struct RouteArgs {
     const void* logits;
@@ -121,21 +122,33 @@ __device__ __forceinline__ double route_sum64(const RouteArgs& a, int64_t t, int
     return sum;
 }
 
-// G lanes per token, V consecutive experts per lane, V <= 16.  K rounds of: largest key of the lanes, the experts
-// that may hold it, the winner.  Without a bias the keys are the logits, exact, and equal ones go to the lowest
-// index.  With one they are the fp32 choices: the experts within the margin of the largest (nearly always just
-// one) are compared in 64 bits.  The weights are formed from the selected experts' logits alone.
+// G lanes per token, V consecutive experts per lane, V <= 16.  Without a bias the keys are the logits, exact, and
+// equal ones go to the lowest index.  With one they are the fp32 choices; experts within the margin of one that is
+// selected (a token in a thousand) are compared in 64 bits.  The weights are formed from the selected experts'
+// logits alone.
 //
-// Bound by the instructions of the K rounds (about 5 V + 30 each for 64 / G tokens a wave) and, below a few thousand
-// tokens, by latency.  16 lanes of 16 experts for E = 256 make a round four tokens' worth of work per wave; a
-// wave per token spends most of a round on the reductions.
+// The selection is K rounds of: largest key of the lanes, the experts that may hold it, the winner; or, for more than
+// 64 experts and K > 4, ranks inside a short list, whose cost hardly grows with K.  us, rounds | list, 8192 tokens,
+// without a bias: E = 64, K = 4: 4.4 | 4.8, 8: 5.6 | 5.6, 16: 7.8 | 14.2 (so 8 lanes have no list); E = 128, K = 4: 4.9 | 5.2,
+// 6: 5.6 | 5.3, 16: 9.5 | 6.6; E = 256, K = 8: 8.2 | 6.3; E = 512, K = 8: 12.6 | 8.0, 16: 19.2 | 9.0.  With a bias E = 256, K = 8:
+// 11.2 | 8.8, in 8 groups, 4 of them kept: 13.2 | 10.5 (8.9 MB: 1.8 us of memory time).
+// Bound by instructions (a round is about 5 V + 30 for 64 / G tokens a wave) and, below a few thousand tokens, by
+// latency (16 experts with K = 2 take 3.4 us).  16 lanes of 16 experts for E = 256 make a round four tokens' worth of
+// work per wave; a wave per token spends most of a round on the reductions.
 template <typename LT, int G, int V, bool SIGMOID, bool BIASED>
 __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
     constexpr int kTokens = 256 / G, kE = G * V;
-    __shared__ uint32_t gkey[kTokens][kRouteMaxGroups];
-    __shared__ uint32_t ckey[kTokens][kE < 2 * G ? 2 * G : kE];
+    __shared__ __attribute__((aligned(16))) uint32_t gkey[kTokens][kRouteMaxGroups];
     __shared__ double wide[kTokens][kRouteMaxGroups];
     __shared__ int chosen[kTokens][kRouteMaxK];
+    // the keys of the group scores, later the list
+    constexpr bool kListed = G >= 16;
+    constexpr int kWords = kE < 2 * G ? 2 * G : kE;
+    static_assert(!kListed || (kWords >= 2 * kRouteList && kRouteList <= kRouteMaxGroups), "rows of shared memory");
+    __shared__ __attribute__((aligned(16))) uint32_t words[kTokens][kWords];
+    auto& ckey = words;
+    auto list = reinterpret_cast<uint64_t (*)[kWords / 2]>(&words[0][0]);
+    __shared__ int listed[kTokens];
     const int tid = threadIdx.x, li = tid % G, slot = tid / G, lane = tid & 63;
     const int64_t t0 = (int64_t)blockIdx.x * kTokens + slot;
     const int64_t t = t0 < a.T ? t0 : a.T - 1;
@@ -295,9 +308,18 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
                 for (int j = 0; j < V; ++j)
                     ckey[slot][e0 + j] = key[j] == 0 ? 0 : (summed && !BIASED ? route_key(s[j]) : key[j]);
                 wave_lds_fence();
+                const float border = route_value(kept_min), beyond = route_value(shut_max);
+                const float apart = 2.0f * route_margin<SIGMOID>(s_max, fmaxf(fabsf(border), fabsf(beyond)));
                 for (int q = 0; q < n_mine; ++q) {
                     const int g = li + q * G;
+                    // far from the border: certain either way
+                    const float own = route_value(gkey[slot][g]);
+                    if (gkey[slot][g] <= 1 || own < border - apart || own > beyond + apart) {
+                        wide[slot][g] = gkey[slot][g] > 1 && own > beyond + apart ? INFINITY : -INFINITY;
+                        continue;
+                    }
                     uint32_t k1 = 0, k2 = 0;
+#pragma unroll 8
                     for (int e = g * gs; e < (g + 1) * gs; ++e) {
                         const uint32_t k = ckey[slot][e];
                         const uint32_t lo = k < k1 ? k : k1;
@@ -308,8 +330,10 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
                     if (k1 > 1) {
                         const float v = route_value(summed && k2 > 1 ? k2 : k1);
                         const uint32_t from = route_key(v - route_margin<SIGMOID>(s_max, v));
-                        for (int e = g * gs; e < (g + 1) * gs; ++e) {
-                            if (ckey[slot][e] <= 1 || ckey[slot][e] < from) continue;
+                        for (int e = g * gs;; ++e) {
+                            // (the lanes meet at the evaluation, one member each)
+                            while (e < (g + 1) * gs && (ckey[slot][e] <= 1 || ckey[slot][e] < from)) ++e;
+                            if (e >= (g + 1) * gs) break;
                             double c = route_score64<SIGMOID>(route_load<LT>(a.logits, t * a.ld + e), m, total);
                             if constexpr (BIASED) c += (double)a.bias[e];
                             if (c > b1) {
@@ -344,6 +368,108 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
         }
     }
 
+    // From a short list: whatever is selected is at least as large as the K-th largest of the lanes' (for 16 lanes, of
+    // their halves') largest keys.  Every expert on the list counts the ones ahead of it, all at once.  A list that
+    // is too long (a row in ascending order, equal logits) is left to the rounds.
+    bool rounds = !kListed || a.K <= 4;
+    if (kListed && !rounds) {
+        constexpr int S = G == 16 ? 2 : 1;
+        uint32_t top[S];
+#pragma unroll
+        for (int h = 0; h < S; ++h) {
+            top[h] = key[h * (V / S)];
+#pragma unroll
+            for (int j = 1; j < V / S; ++j) top[h] = key[h * (V / S) + j] > top[h] ? key[h * (V / S) + j] : top[h];
+            gkey[slot][S * li + h] = top[h];
+        }
+        if (li == 0) listed[slot] = 0;
+#pragma unroll
+        for (int q = 0; q < (kRouteMaxK + G - 1) / G; ++q)
+            if (li + q * G < a.K) chosen[slot][li + q * G] = -1;
+        wave_lds_fence();
+        uint32_t from = 0xffffffffu;
+        int ahead[S] = {};
+#pragma unroll
+        for (int o = 0; o < S * G; o += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(&gkey[slot][o]);
+#pragma unroll
+            for (int h = 0; h < S; ++h) ahead[h] += (w.x > top[h]) + (w.y > top[h]) + (w.z > top[h]) + (w.w > top[h]);
+        }
+#pragma unroll
+        for (int h = 0; h < S; ++h)
+            if (ahead[h] < a.K) from = top[h] < from ? top[h] : from;
+        from = route_min<G>(from);
+        if constexpr (BIASED) {
+            if (from > 1) {
+                const float v = route_value(from);
+                from = route_key(v - route_margin<SIGMOID>(s_max, v));
+            }
+        }
+        from = from < 1 ? 1 : from;
+        int mine_listed = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) mine_listed += key[j] >= from;
+        int at = mine_listed ? atomicAdd(&listed[slot], mine_listed) : 0;  // (any order: ranks do not depend on it)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (key[j] < from) continue;
+            if (at < kRouteList) list[slot][at] = (uint64_t)key[j] << 32 | (uint32_t)(0xffff - (e0 + j));
+            ++at;
+        }
+        wave_lds_fence();
+        const int n = listed[slot];
+        rounds = n > kRouteList;
+        bool doubt = false;
+        if (!rounds) {
+            for (int i = li; i < n; i += G) {
+                const uint64_t own = list[slot][i];
+                uint32_t near_from = 0;
+                if constexpr (BIASED) {
+                    const float v = route_value((uint32_t)(own >> 32));
+                    near_from = route_key(v - route_margin<SIGMOID>(s_max, v));
+                }
+                int before = 0, near = 0;
+#pragma unroll 4
+                for (int o = 0; o < n; ++o) {
+                    const uint64_t other = list[slot][o];
+                    before += other > own;
+                    if constexpr (BIASED) near += (uint32_t)(other >> 32) >= near_from;
+                }
+                if (before < a.K) {
+                    chosen[slot][before] = 0xffff - (int)(uint32_t)own;
+                    // one behind it, and within the margin
+                    if (BIASED && (own >> 32) > 1 && near > before + 1) doubt = true;
+                }
+            }
+        }
+        if constexpr (BIASED) {
+            doubt = (__ballot(doubt) & mine) != 0;
+            if (__any(doubt)) {
+                const double total = SIGMOID ? 1.0 : route_sum64<LT, G>(a, t, li, m);
+                if (doubt) {
+                    for (int i = li; i < n; i += G) {
+                        const int e = 0xffff - (int)(uint32_t)list[slot][i];
+                        wide[slot][i] = route_score64<SIGMOID>(route_load<LT>(a.logits, t * a.ld + e), m, total) + (double)a.bias[e];
+                    }
+                }
+                wave_lds_fence();
+                if (doubt) {
+                    for (int i = li; i < n; i += G) {
+                        const double own = wide[slot][i];
+                        const int e = 0xffff - (int)(uint32_t)list[slot][i];
+                        int before = 0;
+                        for (int o = 0; o < n; ++o) {
+                            const double other = wide[slot][o];
+                            const bool lower = 0xffff - (int)(uint32_t)list[slot][o] < e;
+                            before += other > own || (other == own && lower) || (own != own && (other == other || lower));
+                        }
+                        if (before < a.K) chosen[slot][before] = e;
+                    }
+                }
+            }
+        }
+    }
+    if (__any(rounds))
     for (int k = 0; k < a.K; ++k) {
         uint32_t best = key[0];
 #pragma unroll
@@ -359,7 +485,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
         uint32_t cand = 0;  // this lane's experts that may be the largest
 #pragma unroll
         for (int j = 0; j < V; ++j) cand |= (key[j] >= from ? 1u : 0u) << j;
-        if (top == 0) cand = 0;
+        if (top == 0 || !rounds) cand = 0;
         int at = __ffs(cand) - 1;
         unsigned long long holders = __ballot(cand != 0) & mine;
         if constexpr (BIASED) {
@@ -394,7 +520,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
             for (int j = 0; j < V; ++j) key[j] = j == at ? 0 : key[j];
             chosen[slot][k] = e0 + at;
         }
-        if (top == 0 && li == 0) chosen[slot][k] = -1;
+        if (top == 0 && rounds && li == 0) chosen[slot][k] = -1;
     }
     wave_lds_fence();
 

@@ -508,6 +508,33 @@ def test_routing_tells_choices_apart_that_differ_by_less_than_a_rounding():
         assert torch.equal(idx.cpu().long(), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,k", [(16, 3), (16, 16), (64, 8), (100, 16), (256, 3), (256, 8), (512, 16)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [True, False])
+def test_routing_of_rows_with_an_order(E, k, scoring, biased):
+    """Rows whose largest experts are neighbours, whose experts are equal, or whose scores round to the same in fp32."""
+    N = native()
+    g = torch.Generator().manual_seed(E + k)
+    up = torch.linspace(-2, 2, E)
+    rows = [up, -up, torch.zeros(E), torch.full((E,), 3.0), (up * 4).round(), 20 + up, 20 + up[torch.randperm(E, generator=g)],
+            torch.where(torch.arange(E) % 7 == 3, 1.5, -1.5)]
+    for first in range(0, E, max(k, E // 5)):       # the largest ones side by side, over every border of lanes
+        rows.append(torch.randn(E, generator=g) * 0.1)
+        rows[-1][first:first + k] += 5
+    few = torch.full((E,), float("-inf"))
+    few[E // 2] = few[-1] = few[0] = 0.25
+    x = torch.stack(rows + [few] + [torch.randn(E, generator=g) for _ in range(9)])
+    bias = torch.where(torch.arange(E) % 2 == 0, 0.25, 0.5) if biased else None
+    T = x.shape[0]
+    idx = torch.full((T, k), -7, dtype=torch.int32, device=DEV)
+    gate = torch.full((T, k), -7.0, device=DEV)
+    N.moe_route(x.to(DEV), idx, gate, bias=None if bias is None else bias.to(DEV), scoring=scoring)
+    want, want_gate = O.moe_route(x.double(), k, bias=None if bias is None else bias.double(), scoring=scoring)
+    assert torch.equal(idx.cpu().long(), want)
+    within(gate, want_gate, 2 * route_sums(E) * want_gate, "gate")
+
+
 # ---- permutation ------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,E", [(0, 4), (1, 1), (10, 64), (96, 64), (2048, 8), (2049, 3), (5001, 256), (40000, 1024),
