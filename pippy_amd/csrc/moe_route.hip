@@ -131,7 +131,7 @@ __device__ __forceinline__ double route_sum64(const RouteArgs& a, int64_t t, int
 // 64 experts and K > 4, ranks inside a short list, whose cost hardly grows with K.  us, rounds | list, 8192 tokens,
 // without a bias: E = 64, K = 4: 4.4 | 4.8, 8: 5.6 | 5.6, 16: 7.8 | 14.2 (so 8 lanes have no list); E = 128, K = 4: 4.9 | 5.2,
 // 6: 5.6 | 5.3, 16: 9.5 | 6.6; E = 256, K = 8: 8.2 | 6.3; E = 512, K = 8: 12.6 | 8.0, 16: 19.2 | 9.0.  With a bias E = 256, K = 8:
-// 11.2 | 8.8, in 8 groups, 4 of them kept: 13.2 | 10.5 (8.9 MB: 1.8 us of memory time).
+// 11.2 | 8.8, in 8 groups, 4 of them kept: 13.2 | 9.4 to 10.9 (8.9 MB: 1.8 us of memory time).
 // Bound by instructions (a round is about 5 V + 30 for 64 / G tokens a wave) and, below a few thousand tokens, by
 // latency (16 experts with K = 2 take 3.4 us).  16 lanes of 16 experts for E = 256 make a round four tokens' worth of
 // work per wave; a wave per token spends most of a round on the reductions.
@@ -330,17 +330,23 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
                     if (k1 > 1) {
                         const float v = route_value(summed && k2 > 1 ? k2 : k1);
                         const uint32_t from = route_key(v - route_margin<SIGMOID>(s_max, v));
-                        for (int e = g * gs;; ++e) {
-                            // (the lanes meet at the evaluation, one member each)
-                            while (e < (g + 1) * gs && (ckey[slot][e] <= 1 || ckey[slot][e] < from)) ++e;
-                            if (e >= (g + 1) * gs) break;
-                            double c = route_score64<SIGMOID>(route_load<LT>(a.logits, t * a.ld + e), m, total);
-                            if constexpr (BIASED) c += (double)a.bias[e];
-                            if (c > b1) {
-                                b2 = b1;
-                                b1 = c;
-                            } else if (c > b2) {
-                                b2 = c;
+                        for (int first = g * gs, left = gs; left > 0; first += 32, left -= 32) {
+                            uint32_t may = 0;
+#pragma unroll 8
+                            for (int i = 0; i < (left < 32 ? left : 32); ++i) {
+                                const uint32_t k = ckey[slot][first + i];
+                                may |= (k > 1 && k >= from ? 1u : 0u) << i;
+                            }
+                            for (; may; may &= may - 1) {
+                                const int e = first + __ffs(may) - 1;
+                                double c = route_score64<SIGMOID>(route_load<LT>(a.logits, t * a.ld + e), m, total);
+                                if constexpr (BIASED) c += (double)a.bias[e];
+                                if (c > b1) {
+                                    b2 = b1;
+                                    b1 = c;
+                                } else if (c > b2) {
+                                    b2 = c;
+                                }
                             }
                         }
                     }
@@ -348,11 +354,16 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
                 }
                 wave_lds_fence();
                 unsigned long long again = 0;
-                for (int g = 0; g < a.n_group; ++g) {
-                    const double own = wide[slot][g];
+                for (int q = 0; q * G < a.n_group; ++q) {
+                    const int g = li + q * G;
+                    const double own = g < a.n_group ? wide[slot][g] : 0.0;
                     int ahead = 0;
-                    for (int o = 0; o < a.n_group; ++o) ahead += wide[slot][o] > own || (wide[slot][o] == own && o < g);
-                    if (ahead < a.topk_group) again |= 1ull << g;
+#pragma unroll 8
+                    for (int o = 0; o < a.n_group; ++o) {
+                        const double other = wide[slot][o];
+                        ahead += other > own || (other == own && o < g);
+                    }
+                    again |= ((__ballot(g < a.n_group && ahead < a.topk_group) & mine) >> (lane & ~(G - 1))) << (q * G);
                 }
                 if (doubt) open = again;
             }
@@ -458,6 +469,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
                         const double own = wide[slot][i];
                         const int e = 0xffff - (int)(uint32_t)list[slot][i];
                         int before = 0;
+#pragma unroll 4
                         for (int o = 0; o < n; ++o) {
                             const double other = wide[slot][o];
                             const bool lower = 0xffff - (int)(uint32_t)list[slot][o] < e;
