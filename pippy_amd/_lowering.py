@@ -1164,7 +1164,7 @@ def lower_stage_module(submod: nn.Module, why: Optional[List[str]] = None, for_k
                     or (isinstance(m, nn.MultiheadAttention) and m.dropout > 0 and m.training)]
             if live and "dropout" not in reason:
                 shown = ", ".join(live[:3]) + (", ..." if len(live) > 3 else "")
-                reason = (f"dropout with p > 0 in training mode ({shown}): the launch lists hold no dropout; "
+                reason = (f"dropout with p > 0 in training mode ({shown}): the launch lists hold no dropout layers; "
                           f"set p = 0 or build the stage in eval mode.  The recogniser says: {reason}")
             why.append(reason)
         return None

@@ -51,7 +51,8 @@ __host__ __device__ inline int64_t plan_blocks128(int64_t T, int64_t n_seq) { re
 // without one.  Entries {first row of the sequence, its length, block index, 0}, dearest blocks first: under a causal
 // mask a block costs as many steps as its index says, without one as its sequence has blocks.  A counting sort over
 // that; a wave takes a sequence at a time, its lanes the blocks.  The order inside a class is left to the atomics,
-// since it only says which work-group does what.
+// since it only says which work-group does what.  Bound by latency (two passes over the bounds, a scan, barriers):
+// 4.5 us for 4001 rows in 13 sequences as for 16384 in 3; one work-group for all lists took 6.1.
 __global__ __launch_bounds__(kPlanThreads) void attn_packed_plan_kernel(const int32_t* __restrict__ cu, int n_seq,
                                                                         int T, int32_t* __restrict__ plan,
                                                                         int cap64, int cap128) {
@@ -166,7 +167,11 @@ struct PackedTileLoader {
 
 // ---- forward ------------------------------------------------------------------------------------
 // A work-group owns 64 query rows of one head and walks the keys in blocks of 64.  Its 4 waves are 2 groups of
-// 32 queries x 2 halves of every key block; the two waves of a group merge once, through LDS.
+// 32 queries x 2 halves of every key block; the two waves of a group merge once, through LDS: a sequence's last
+// block takes half as long as with a wave over all its keys, and short sequences fill twice the SIMDs.  Bound by
+// the longest work-group's chain of steps (about 0.5 us each: loads, scores, exponentials, the second product).
+// 37 rows, 12 heads of 64: 4.5 us; [4001 rows in 13 sequences, 12 heads], no mask: 16.5 us; [4096
+// rows in 11 documents, 12 heads], causal: 14.6 us.
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -318,6 +323,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(c
 
 // The form for long sequences: a work-group owns 128 query rows, 32 per wave, and every wave walks all keys, in
 // blocks of 64: twice the products per staged block and barrier, half the passes over keys and values, and no merge.
+// Bound by the matrix cores beside the exponentials: causal [8192 rows, 32 query and 8 key / value heads of 128] 519 us =
+// 1060 TFLOP/s of the products it forms (a library product of 8192^3 reaches 1211), 57 % of the cycles in the matrix
+// cores, no LDS conflicts; 16384 rows in 3 sequences, 870 us.
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd128_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -487,7 +495,8 @@ __device__ __forceinline__ float packed_delta(const uint16_t* qp, const uint16_t
 }
 
 // A work-group owns 64 query rows (2 groups of 32 queries x 2 halves of every key block) and hands the dK / dV
-// kernel the row sums D = sum_j P dP.
+// kernel the row sums D = sum_j P dP.  Bound like the forward's form of 64 rows: [4096 rows in 11 documents, 12 heads of
+// 64], causal: 19 us.
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -615,7 +624,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         }
 }
 
-// The form for long sequences: 128 query rows, 32 per wave, every wave over all keys (see the forward).
+// The form for long sequences: 128 query rows, 32 per wave, every wave over all keys (see the forward).  Three
+// products per pair of blocks: 224 us for causal [8192 rows in 5 documents, 32 query and 8 key / value heads of 128].
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -747,7 +757,8 @@ __global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const Pac
 // ---- backward: dK, dV ---------------------------------------------------------------------------
 // A work-group owns 64 keys of one key / value head and walks the query blocks that see them, one query head of
 // the group after the other, so the sums over a group have a fixed order.  4 waves: 2 groups of 32 keys x 2
-// halves of every query block.  Head dimension 64.
+// halves of every query block.  Head dimension 64.  [4096 rows in 11 documents, 12 heads], causal: 23 us, bound by the
+// chain of the keys with the most queries behind them.
 template <bool CAUSAL>
 __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const PackedArgs a) {
     constexpr int D = 64;
@@ -925,7 +936,9 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
 // Head dimension 128: 8 waves per work-group, so that two waves share a SIMD and one's products run beside the
 // other's exponentials; to fit the registers of that the value rows stay in LDS.  KB blocks of 64 keys per
 // work-group: 2, as 4 groups of 32 keys x 2 parts of a step of 64 queries, or 1, as 2 groups x 4 parts of 128
-// queries: twice the work-groups with half the steps each, for launches that would not fill the CUs.
+// queries: twice the work-groups with half the steps each, for launches that would not fill the CUs.  Four
+// products per pair of blocks and the exponentials again; 370 us for causal [8192 rows in 5 documents, 32 query and 8
+// key / value heads], 47 % of the cycles in the matrix cores: two waves per SIMD is what the registers allow.
 template <int D, bool CAUSAL, int KB>
 __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = 2;

@@ -91,6 +91,8 @@ struct DropoutVec<float> {
     static __device__ __forceinline__ void store1(void* p, int64_t i, float v) { static_cast<float*>(p)[i] = v; }
 };
 
+// Bound by HBM: bf16 [16384, 4096] with a residual 69 to 75 us (5.4 to 5.8 TB/s over 403 MB), without one 45 us (5.9 TB/s);
+// the generator's 20 wide products per 8 elements hide behind that.  [1021, 768]: 3 us, latency.
 constexpr int kDropoutGroups = 2;  // groups of 8 elements per lane: their loads are all in flight at once
 
 template <typename ET, bool FLAT, bool RESID>

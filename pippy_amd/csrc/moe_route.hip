@@ -576,7 +576,8 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
 // dgate_k is given, or <dout[t], y[pos(t, k)]> over the expert rows.
 //
 // One wave per token; lane k < K holds slot k.  Bound by the expert rows: per chunk of 512 columns the loads of the
-// gradient row and of all K expert rows go out together.
+// gradient row and of all K expert rows go out together.  [4093 tokens, 6 of 64 experts, 1024 columns]: 13.2 us, 4.5
+// TB/s over 59 MB.
 struct RouteBwdArgs {
     const void* logits;
     int64_t ld, T;

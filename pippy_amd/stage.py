@@ -364,7 +364,7 @@ class PipelineStageBase:
         if self._mode_bound_dropouts and any(m.training for m in self._mode_bound_dropouts):
             raise RuntimeError(
                 f"{self.log_prefix} was lowered to launch lists in eval mode, where its dropout layers (p > 0) do "
-                "nothing, and its module is in training mode now: the launch lists hold no dropout.  Set the mode "
+                "nothing, and its module is in training mode now: the launch lists hold no dropout layers.  Set the mode "
                 "before the stage is built (a stage built in training mode with p > 0 runs through torch "
                 "autograd), or set the dropout probabilities to 0")
         sp = self._stage_program()
