@@ -527,7 +527,8 @@ int pp_attn_bwd(const pp_attn_desc* desc, pp_stream stream);
  * backward; the backward's row sums of P dP).  D 64 or 128.  scale > 0.  Softmax statistics and all sums are fp32;
  * P and dS are rounded to bf16 as operands of their products.  No atomics: the same bits on every run.
  * A non-finite value row reaches, besides the queries that see it, earlier queries of its block of rows (0 * NaN
- * inside a matrix product), never another sequence.
+ * inside a matrix product), and in the backward a non-finite row of d_o, q or k the other rows of its blocks; never
+ * another sequence.
  *
  * The plan says which blocks of rows there are, the dearest first.  pp_attn_packed_plan builds it on the device from
  * cu_seqlens (one small launch, no host synchronisation); every layer and both directions of a batch share it.  The

@@ -639,7 +639,8 @@ def _dropout_rows(x, y, resid):
         return 1, n, n, n, n
     _need(len(shape) == 2 and all(t is None or t.stride(1) == 1 for t in (x, y, resid)),
           "dropout: contiguous tensors, or two-dimensional ones with contiguous rows")
-    ld = [0 if t is None else max(t.stride(0), shape[1]) for t in (x, resid, y)]
+    ld = [0 if t is None else t.stride(0) if shape[0] > 1 else shape[1] for t in (x, resid, y)]
+    _need(all(t is None or n >= shape[1] for t, n in zip((x, resid, y), ld)), "dropout: rows that overlap (an expanded tensor)")
     return (shape[0], shape[1], *ld)
 
 

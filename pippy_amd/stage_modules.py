@@ -1185,8 +1185,8 @@ class MoELayer(_MoEFeedForward, LlamaLayer):
         LlamaLayer.__init__(self, dim, n_heads, ffn, eps=eps, rope_theta=rope_theta, dtype=dtype,
                             init_std=init_std, n_kv_heads=n_kv_heads)
         del self.mlp
-        if (top_k, scoring, n_group, norm_topk, routed_scale, balance_bias) != (2, "softmax", 1, True, 1.0, False) or \
-                n_experts > 64:
+        if (top_k, scoring, n_group, topk_group, group_score, norm_topk, routed_scale, balance_bias) != \
+                (2, "softmax", 1, 1, "max", True, 1.0, False) or n_experts > 64:
             if scoring not in N.MOE_SCORING or group_score not in N.MOE_GROUP_SCORE:
                 raise ValueError(f"scoring {scoring!r}, group_score {group_score!r}; known: {sorted(N.MOE_SCORING)}, "
                                  f"{sorted(N.MOE_GROUP_SCORE)}")

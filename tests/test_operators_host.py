@@ -7,6 +7,7 @@ import torch
 
 from oracle import ops as O
 from pippy_amd import _native as N
+from pippy_amd.stage_modules import MoELayer
 
 
 # ---- the oracle -----------------------------------------------------------------------------------
@@ -49,6 +50,24 @@ def test_routing_agrees_with_topk_and_with_the_top2_router():
     x[1, 1:] = float("-inf")
     idx, gate = O.moe_route(x, 2)
     assert idx[:2].tolist() == [[-1, -1], [0, -1]] and gate[:2].tolist() == [[0, 0], [1, 0]]
+
+
+def test_dropout_refuses_rows_that_overlap():
+    """Expanded and overlapping rows have no leading dimension that the kernels could take."""
+    x = torch.zeros(4, 16)
+    for bad in (torch.zeros(1, 16).expand(4, 16), torch.zeros(64).as_strided((4, 16), (8, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            N._dropout_rows(bad, x, None)
+        with pytest.raises(ValueError, match="overlap"):
+            N._dropout_rows(x, x, bad)
+    assert N._dropout_rows(torch.zeros(4, 24)[:, :16], x, None) == (4, 16, 24, 0, 16)
+    assert N._dropout_rows(torch.zeros(4, 24)[:1, :16], x[:1], None) == (1, 16, 16, 16, 16)
+
+
+def test_moe_layer_refuses_groups_that_do_not_exist():
+    for bad in (dict(topk_group=3), dict(group_score="mean"), dict(n_group=3), dict(n_group=4, topk_group=5), dict(top_k=9)):
+        with pytest.raises(ValueError):
+            MoELayer(128, 2, 16, 8, **bad)
 
 
 def test_philox_known_answers():
