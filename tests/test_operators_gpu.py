@@ -221,6 +221,41 @@ def test_packed_attention_of_separate_tensors_and_many_short_sequences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[1, 2], [2, 1, 3, 2], [8, 33, 64]])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_packed_attention_query_gradient_of_few_keys(lens, causal, D):
+    """With one block of keys the row sums in dS are those of P dP: the rounding of the output does not reach dQ.
+    What is left: dS rounded to bf16 (2^-8 of each term of the sum over the keys), dQ rounded to bf16, and 2^-16 of every
+    term of dS for the fp32 exponentials and sums (scores up to 2^5: P is off by 2^5 2^-22, the sums over D by D 2^-24)."""
+    N = native()
+    H, T = 5, sum(lens)
+    g = torch.Generator().manual_seed(T + D)
+    q, k, v, do = (torch.randn(T, H, D, generator=g).to(torch.bfloat16) for _ in range(4))
+    cu = torch.tensor([0] + lens).cumsum(0).int()
+    qd, kd, vd, dod = (t.to(DEV) for t in (q, k, v, do))
+    o, dq, dk, dv = (torch.empty_like(qd) for _ in range(4))
+    lse, delta = (torch.empty(H, T, device=DEV) for _ in range(2))
+    plan = N.attn_packed_plan(cu.to(DEV), T)
+    N.attn_packed_fwd(qd, kd, vd, o, lse, plan, causal=causal)
+    N.attn_packed_bwd(qd, kd, vd, o, lse, dod, dq, dk, dv, delta, plan, causal=causal)
+    scale = D ** -0.5
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        Q, K, V, dO = (t[a:b].double().transpose(0, 1) for t in (q, k, v, do))
+        S = Q @ K.transpose(1, 2) * scale
+        if causal:
+            S = S.masked_fill(torch.ones(b - a, b - a, dtype=torch.bool).triu(1), float("-inf"))
+        P = torch.softmax(S, -1)
+        dP = dO @ V.transpose(1, 2)
+        row = (P * dP).sum(-1, keepdim=True)
+        dS = P * (dP - row)
+        want = dS @ K * scale
+        noise = P * (dP.abs() + (P * dP.abs()).sum(-1, keepdim=True))
+        bound = scale * (U * dS.abs() + 2.0 ** -16 * noise) @ K.abs() + U * want.abs()
+        within(dq[a:b].transpose(0, 1), want, 1.01 * bound + 1e-30, "dq")
+
+
+@pytest.mark.gpu
 def test_packed_attention_gradients_agree_with_differences():
     """The directional derivative of <o, do> from the kernel's gradients against central differences of the
     definition in 64 bits."""
