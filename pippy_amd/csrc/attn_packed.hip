@@ -780,10 +780,24 @@ __global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const Pac
 }
 
 // ---- backward: dK, dV ---------------------------------------------------------------------------
+// A lane holds 16 queries' scores of one key, so log-sum-exp and delta differ from element to element.  They enter the
+// products instead, as one more small one: a query's number as three bf16 terms without a remainder (8 bits each) in its
+// operand row, against ones.  That is one 4-byte LDS read per lane and statistic where there were four broadcast
+// 16-byte ones (a quarter of the kernel's LDS cycles, which bound it beside the matrix cores) and 32 vector
+// instructions less: one document of 832 tokens 17.8 -> 14.1 us, [4096 rows, 16 heads of 64] 95 -> 85, [8192, 32 / 8 heads
+// of 128] 1093 -> 1026.
+typedef short packed_s16x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ packed_s16x4_t packed_three_parts(float x) {
+    const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u), rest = x - hi;
+    const float mid = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+    const uint2 w = make_uint2((__float_as_uint(hi) >> 16) | __float_as_uint(mid), __float_as_uint(rest - mid) >> 16);
+    return __builtin_bit_cast(packed_s16x4_t, w);
+}
+
 // A work-group owns 64 keys of one key / value head and walks the query blocks that see them, one query head of
 // the group after the other, so the sums over a group have a fixed order.  4 waves: 2 groups of 32 keys x 2
-// halves of every query block.  Head dimension 64.  [4096 rows in 11 documents, 12 heads], causal: 23 us, bound by the
-// chain of the keys with the most queries behind them.
+// halves of every query block.  Head dimension 64.  [4096 rows in 11 documents, 12 heads], causal: 20.5 us, bound by the
+// chain of the keys with the most queries behind them (0.85 us a step).
 template <bool CAUSAL>
 __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const PackedArgs a) {
     constexpr int D = 64;
@@ -852,6 +866,9 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
             dkacc[t][e] = 0.f;
         }
     const float c = a.scale * kLog2e;
+    // S - lse / scale and dP - delta come out of the products themselves (see packed_three_parts)
+    const float lse_f = lh == 0 ? -1.0f / a.scale : 0.f, delta_f = lh == 0 ? -1.0f : 0.f;
+    const packed_s16x4_t ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80};
 
     // one block of 64 queries from query qb0 on; MASKED: the diagonal block of a causal mask
     auto step = [&](auto masked_c, const uint16_t* Qs, int qb0) __attribute__((always_inline)) {
@@ -871,17 +888,13 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qfr, kf[ks], sacc, 0, 0, 0);
             dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ofr, vf[ks], dpacc, 0, 0, 0);
         }
+        sacc = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(packed_three_parts(lse_s[32 * half + l32] * lse_f), ones, sacc, 0, 0, 0);
+        dpacc = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(packed_three_parts(delta_s[32 * half + l32] * delta_f), ones, dpacc, 0, 0, 0);
         // element v: query qb0 + 32 half + 8 (v / 4) + 4 lh + v % 4, key kvi.  A query past the end has zero rows, a
         // zero log-sum-exp and a zero delta: P = 1 meets dO = 0, dS = 0.
         float pv[16], dsv[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 l4 = *reinterpret_cast<const float4*>(lse_s + 32 * half + 8 * g + 4 * lh);
-            const float lq4[4] = {l4.x * kLog2e, l4.y * kLog2e, l4.z * kLog2e, l4.w * kLog2e};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                pv[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sacc[4 * g + e], c, -lq4[e]));
-        }
+        for (int v = 0; v < 16; ++v) pv[v] = __builtin_amdgcn_exp2f(sacc[v] * c);
         if constexpr (decltype(masked_c)::value) {
             const int lim = kvi - qb0 - 32 * half - 4 * lh;  // earlier queries do not see this key
 #pragma unroll
@@ -889,12 +902,7 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
                 if (8 * (v >> 2) + (v & 3) < lim) pv[v] = 0.f;
         }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 d4 = *reinterpret_cast<const float4*>(delta_s + 32 * half + 8 * g + 4 * lh);
-            const float dq4[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dsv[4 * g + e] = pv[4 * g + e] * (dpacc[4 * g + e] - dq4[e]);
-        }
+        for (int v = 0; v < 16; ++v) dsv[v] = pv[v] * dpacc[v];
 #pragma unroll
         for (int gp = 0; gp < 2; ++gp) {
             const bf16x8_t pb = pack8(pv + 8 * gp);
@@ -962,8 +970,8 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
 // other's exponentials; to fit the registers of that the value rows stay in LDS.  KB blocks of 64 keys per
 // work-group: 2, as 4 groups of 32 keys x 2 parts of a step of 64 queries, or 1, as 2 groups x 4 parts of 128
 // queries: twice the work-groups with half the steps each, for launches that would not fill the CUs.  Four
-// products per pair of blocks and the exponentials again; 370 us for causal [8192 rows in 5 documents, 32 query and 8
-// key / value heads], 47 % of the cycles in the matrix cores: two waves per SIMD is what the registers allow.
+// products per pair of blocks and the exponentials again; 333 us for causal [8192 rows in 5 documents, 32 query and 8
+// key / value heads].  Bound by LDS reads beside the matrix cores; two waves per SIMD is what the registers allow.
 template <int D, bool CAUSAL, int KB>
 __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = 2;
@@ -1035,6 +1043,9 @@ __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const Pack
             dkacc[t][e] = 0.f;
         }
     const float c = a.scale * kLog2e;
+    // S - lse / scale and dP - delta come out of the products themselves (see packed_three_parts)
+    const float lse_f = lh == 0 ? -1.0f / a.scale : 0.f, delta_f = lh == 0 ? -1.0f : 0.f;
+    const packed_s16x4_t ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80};
     const uint16_t* Vs = Vl + (grp >> 1) * kOperand;
     const int vrow = 32 * (grp & 1) + l32;
     const int qblk = part >> 1, half = part & 1;          // this wave's 32 queries of a step
@@ -1042,7 +1053,7 @@ __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const Pack
     auto step = [&](auto masked_c, const uint16_t* st, int qb0) __attribute__((always_inline)) {
         const uint16_t* Qs = st + qblk * kOperand;
         const uint16_t* Os = st + (QB + qblk) * kOperand;
-        const float* lse_s = reinterpret_cast<const float*>(st + kStats) + 64 * qblk + 32 * half + 4 * lh;
+        const float* lse_s = reinterpret_cast<const float*>(st + kStats) + 64 * qblk + 32 * half;
         const float* delta_s = lse_s + 64 * QB;
         f32x16_t sacc, dpacc;
 #pragma unroll
@@ -1055,21 +1066,17 @@ __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const Pack
             const bf16x8_t qfr = read_row_frag<swz_packed>(Qs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qfr, kf[ks], sacc, 0, 0, 0);
         }
+        sacc = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(packed_three_parts(lse_s[l32] * lse_f), ones, sacc, 0, 0, 0);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const bf16x8_t ofr = read_row_frag<swz_packed>(Os + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             const bf16x8_t vfr = read_row_frag<swz_packed>(Vs + (ks / 4) * kTile, vrow, 2 * (ks % 4) + lh);
             dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ofr, vfr, dpacc, 0, 0, 0);
         }
+        dpacc = __builtin_amdgcn_mfma_f32_32x32x8bf16_1k(packed_three_parts(delta_s[l32] * delta_f), ones, dpacc, 0, 0, 0);
         float pv[16], dsv[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 l4 = *reinterpret_cast<const float4*>(lse_s + 8 * g);
-            const float lq4[4] = {l4.x * kLog2e, l4.y * kLog2e, l4.z * kLog2e, l4.w * kLog2e};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                pv[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(sacc[4 * g + e], c, -lq4[e]));
-        }
+        for (int v = 0; v < 16; ++v) pv[v] = __builtin_amdgcn_exp2f(sacc[v] * c);
         if constexpr (decltype(masked_c)::value) {
             const int lim = kvi - qb0 - 32 * part - 4 * lh;  // earlier queries do not see this key
 #pragma unroll
@@ -1077,12 +1084,7 @@ __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const Pack
                 if (8 * (v >> 2) + (v & 3) < lim) pv[v] = 0.f;
         }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 d4 = *reinterpret_cast<const float4*>(delta_s + 8 * g);
-            const float dq4[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dsv[4 * g + e] = pv[4 * g + e] * (dpacc[4 * g + e] - dq4[e]);
-        }
+        for (int v = 0; v < 16; ++v) dsv[v] = pv[v] * dpacc[v];
 #pragma unroll
         for (int gp = 0; gp < 2; ++gp) {
             const bf16x8_t pb = pack8(pv + 8 * gp);
