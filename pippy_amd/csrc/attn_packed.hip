@@ -171,7 +171,7 @@ struct PackedTileLoader {
 // block takes half as long as with a wave over all its keys, and short sequences fill twice the SIMDs.  Bound by
 // the longest work-group's chain of steps (about 0.5 us each: loads, scores, exponentials, the second product).
 // 37 rows, 12 heads of 64: 4.5 us; [4001 rows in 13 sequences, 12 heads], no mask: 16.5 us; [4096
-// rows in 11 documents, 12 heads], causal: 14.6 us.
+// rows in 11 documents, 12 heads], causal: 14.1 us.
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(c
 // blocks of 64: twice the products per staged block and barrier, half the passes over keys and values, and no merge.
 // Bound by the matrix cores beside the exponentials: causal [8192 rows, 32 query and 8 key / value heads of 128] 519 us =
 // 1060 TFLOP/s of the products it forms (a library product of 8192^3 reaches 1211), 57 % of the cycles in the matrix
-// cores, no LDS conflicts; 16384 rows in 3 sequences, 870 us.
+// cores, no LDS conflicts; 16384 rows in 3 sequences, 783 to 870 us.
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd128_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -650,7 +650,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
 }
 
 // The form for long sequences: 128 query rows, 32 per wave, every wave over all keys (see the forward).  Three
-// products per pair of blocks: 224 us for causal [8192 rows in 5 documents, 32 query and 8 key / value heads of 128].
+// products per pair of blocks: 213 us for causal [8192 rows in 5 documents, 32 query and 8 key / value heads of 128].
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -971,7 +971,7 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
 // work-group: 2, as 4 groups of 32 keys x 2 parts of a step of 64 queries, or 1, as 2 groups x 4 parts of 128
 // queries: twice the work-groups with half the steps each, for launches that would not fill the CUs.  Four
 // products per pair of blocks and the exponentials again; 333 us for causal [8192 rows in 5 documents, 32 query and 8
-// key / value heads].  Bound by LDS reads beside the matrix cores; two waves per SIMD is what the registers allow.
+// key / value heads], 57 % of the cycles in the matrix cores.  Bound by LDS reads beside those; two waves per SIMD is what the registers allow.
 template <int D, bool CAUSAL, int KB>
 __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = 2;
