@@ -971,7 +971,8 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
 // work-group: 2, as 4 groups of 32 keys x 2 parts of a step of 64 queries, or 1, as 2 groups x 4 parts of 128
 // queries: twice the work-groups with half the steps each, for launches that would not fill the CUs.  Four
 // products per pair of blocks and the exponentials again; 333 us for causal [8192 rows in 5 documents, 32 query and 8
-// key / value heads], 57 % of the cycles in the matrix cores.  Bound by LDS reads beside those; two waves per SIMD is what the registers allow.
+// key / value heads], 57 % of the cycles in the matrix cores.  Bound by LDS reads beside those; two waves per SIMD is
+// what the registers allow.
 template <int D, bool CAUSAL, int KB>
 __global__ __launch_bounds__(512, 2) void attn_packed_bwd_dkv8_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = 2;
@@ -1166,8 +1167,9 @@ static int packed_check(const char* who, const pp_attn_packed_desc* d, bool bwd)
                     (long long)d->n_seq, (long long)d->H, (long long)d->Hkv);
     if (d->D != 64 && d->D != 128)
         return fail(PP_ERR_UNSUPPORTED, "%s: head_dim %lld (64 and 128 are built)", who, (long long)d->D);
-    if (!(d->scale > 0.f) || !(d->scale < INFINITY))
-        return fail(PP_ERR_INVALID, "%s: scale must be positive and finite", who);
+    // (log-sum-exp / scale is formed in fp32)
+    if (!(d->scale >= 0x1p-64f) || !(d->scale <= 0x1p64f))
+        return fail(PP_ERR_INVALID, "%s: scale must be positive and finite, between 2^-64 and 2^64", who);
     const struct { const void* p; int64_t stride, width; const char* name; bool need; } rows[] = {
         {d->q, d->stride_q, d->H * d->D, "q", true},     {d->k, d->stride_k, d->Hkv * d->D, "k", true},
         {d->v, d->stride_v, d->Hkv * d->D, "v", true},   {d->o, d->stride_o, d->H * d->D, "o", true},

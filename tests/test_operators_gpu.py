@@ -172,6 +172,14 @@ def test_packed_attention_with_large_scores_and_a_scale_of_the_callers(D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale", [2.0 ** -60, 1e-3, 4.0])
+def test_packed_attention_with_nearly_equal_and_nearly_single_weights(D, scale):
+    cu = [0, 1, 65, 200]
+    Packed(cu, 200, 4, 2, D, seed=9).run(True, scale=scale).check(True, scale=scale)
+
+
+@pytest.mark.gpu
 def test_packed_attention_sequences_do_not_see_each_other():
     cu = [0, 50, 130, 300]
     clean = Packed(cu, 300, 4, 4, 64, seed=5).run(True)

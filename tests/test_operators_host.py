@@ -124,6 +124,11 @@ def test_packed_attention_refuses(change, match):
     refused(N.lib().pp_attn_packed_fwd(packed(**change), None), match)
 
 
+@pytest.mark.parametrize("change,match", [(dict(scale=1e-30), "scale"), (dict(scale=1e30), "scale"), (dict(H=2 ** 18), "shape")])
+def test_packed_attention_refuses_sizes_beyond_its_arithmetic(change, match):
+    refused(N.lib().pp_attn_packed_fwd(packed(**change), None), match)
+
+
 @pytest.mark.parametrize("change,match", [
     (dict(d_o=None), "d_o must"), (dict(dq=A + 4), "dq must"), (dict(stride_dk=120), "stride"), (dict(delta=None), "null"),
 ])
