@@ -1014,13 +1014,46 @@ def _fuse_column_sums(b: "Builder", prog: MicrobatchProgram) -> None:
                 op.p[2], op.j[1] = ws.data_ptr(), n_part
 
 
+class LiveBuffers:
+    """Buffers of a stage's modules that its launch lists read by address and a training loop updates between steps (a
+    router's balancing bias).
+
+    Every buffer has one storage on the device for the life of the stage.  The tensor that the module holds when the stage
+    is built moves into it (the tensor object stays, as parameters stay when they move into the arena), so an update in
+    place through any reference to it is what the next kernel reads.  Whatever the module holds in its place later (an
+    assignment, ``load_state_dict(assign=True)``, ``module.to``) is copied into the storage at the beginning of every step."""
+
+    def __init__(self, blocks: Sequence[nn.Module], device: torch.device):
+        self._entries: Dict[Tuple[int, str], Tuple[nn.Module, str, torch.Tensor]] = {}
+        for blk in blocks:
+            for module, name, shape in getattr(blk, "_pp_live_buffers", lambda: [])():
+                storage = torch.empty(shape, dtype=torch.float32, device=device)
+                self._entries[(id(module), name)] = (module, name, storage)
+        self.follow()
+        for module, name, storage in self._entries.values():
+            getattr(module, name).data = storage
+
+    def storage(self, module: nn.Module, name: str) -> torch.Tensor:
+        return self._entries[(id(module), name)][2]
+
+    def follow(self) -> None:
+        for module, name, storage in self._entries.values():
+            now = getattr(module, name, None)
+            if not isinstance(now, torch.Tensor) or now.shape != storage.shape:
+                raise RuntimeError(f"{name} must be a tensor of shape {list(storage.shape)}, not "
+                                   f"{list(now.shape) if isinstance(now, torch.Tensor) else now}")
+            if now.data_ptr() != storage.data_ptr() or now.dtype != storage.dtype or now.stride() != storage.stride():
+                storage.copy_(now.detach())
+
+
 class StageProgram:
     """All microbatch programs of one stage plus its arenas and shared buffers."""
 
     def __init__(self, blocks: Sequence[nn.Module], module: nn.Module, device, training: bool,
                  split_backward: bool, fused_accumulate: bool, is_first: bool, is_last: bool,
-                 dropout_seed: int = 0):
+                 dropout_seed: int = 0, live_buffers: Optional["LiveBuffers"] = None):
         self.blocks = list(blocks)
+        self.live_buffers = live_buffers
         self.dropout_seed = dropout_seed
         self.dropout_mode: Tuple[bool, ...] = ()   # which blocks with dropout were in training mode when lowered
         self._rng: Dict[int, torch.Tensor] = {}
@@ -1070,6 +1103,10 @@ class StageProgram:
         if t is None:
             t = self._rng[mb] = torch.tensor([self.dropout_seed, mb << 32], dtype=torch.int64, device=self.device)
         return t
+
+    def live_buffer(self, module: nn.Module, name: str) -> torch.Tensor:
+        """Where the launch lists read buffer ``name`` of ``module`` (see ``LiveBuffers``)."""
+        return self.live_buffers.storage(module, name)
 
     def ones_f32(self, n: int) -> torch.Tensor:
         """A [1, n] row of ones (the left operand that turns an fp32 GEMM into a column sum)."""

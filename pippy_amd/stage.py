@@ -129,6 +129,7 @@ class PipelineStageBase:
         # blocks with a dropout of their own, which runs inside the launch lists while they are in training mode
         self._dropout_blocks = [blk for blk in self._blocks or ()
                                 if isinstance(getattr(blk, "dropout", None), float) and blk.dropout > 0]
+        self._live_buffers = P.LiveBuffers(self._blocks or (), self.device)
         self._program: Optional[P.StageProgram] = None
         #: why this stage runs through torch autograd instead of HIP launch lists (None: it is native)
         self.eager_reason: Optional[str] = None
@@ -198,6 +199,7 @@ class PipelineStageBase:
         """Resets per-step state (reference ``_PipelineStage.py:343-366``)."""
         if self._program is not None:
             self._program.arena.refresh_transposed()
+        self._live_buffers.follow()
         self.fwd_chunk_id = 0
         self.bwd_chunk_id = 0
         self.bwd_weight_chunk_id = 0
@@ -217,7 +219,7 @@ class PipelineStageBase:
                                            split_backward=self.split_backward,
                                            fused_accumulate=self.fused_accumulate,
                                            is_first=self.is_first, is_last=self.is_last,
-                                           dropout_seed=self._dropout_seed())
+                                           dropout_seed=self._dropout_seed(), live_buffers=self._live_buffers)
             self._publish_grad_views()
         elif self._program.training != self.has_backward or \
                 self._program.split_backward != self.split_backward:

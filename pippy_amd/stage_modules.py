@@ -34,6 +34,10 @@ class NativeBlock(nn.Module):
         """Parameters whose gradient is added straight into the fp32 accumulator."""
         return []
 
+    def _pp_live_buffers(self) -> List[Tuple[nn.Module, str, Tuple[int, ...]]]:
+        """(module, buffer name, shape) of the fp32 buffers that the launch lists read and a training loop updates."""
+        return []
+
 
 def _as2d(t: torch.Tensor) -> torch.Tensor:
     return t.reshape(-1, t.shape[-1])
@@ -1067,7 +1071,8 @@ class _MoEFeedForward:
         if how is None:
             b.f(P.op_moe_router(logits, idx, gate, E))
         else:
-            b.f(P.op_moe_route(logits, idx, gate, E, bias=self._balance_bias_on(b.device), **how))
+            bias = b.sp.live_buffer(self.block_sparse_moe, "balance_bias") if self._pp_live_buffers() else None
+            b.f(P.op_moe_route(logits, idx, gate, E, bias=bias, **how))
         seg = b.act("seg_start", (E + 1,), torch.int32)
         row_src = b.act("row_src", (R,), torch.int32)
         pos = b.act("pos", (R,), torch.int32)
@@ -1170,7 +1175,8 @@ class MoELayer(_MoEFeedForward, LlamaLayer):
     ``topk_group`` / ``group_score`` ("max", "top2") keep the experts of the best groups only; ``norm_topk`` renormalises
     the weights; ``routed_scale`` multiplies them; ``balance_bias=True`` adds the fp32 buffer
     ``block_sparse_moe.balance_bias`` [n_experts] to the scores for the selection (no gradient: a training loop updates
-    it in place from the expert loads).  See ``pp_moe_route``.
+    it from the expert loads, in place or by assigning another tensor; a step routes by what the module holds when it
+    begins).  See ``pp_moe_route``.
 
     ``forced_routing`` (a list of int64 [tokens, 2] tensors, one per forward call, consumed in
     order) overrides the expert selection of the torch statement; a comparison against a lower
@@ -1210,12 +1216,9 @@ class MoELayer(_MoEFeedForward, LlamaLayer):
     def _balance_bias(self):
         return getattr(self.block_sparse_moe, "balance_bias", None)
 
-    def _balance_bias_on(self, device):
-        """The bias where the launch lists read it: the module's own buffer, fp32 on the device."""
-        bias = self._balance_bias()
-        if bias is not None and (bias.device != device or bias.dtype != torch.float32):
-            bias = self.block_sparse_moe.balance_bias = bias.to(device=device, dtype=torch.float32)
-        return bias
+    def _pp_live_buffers(self):
+        moe = self.block_sparse_moe
+        return [(moe, "balance_bias", (self.n_experts,))] if "balance_bias" in moe._buffers else []
 
     @property
     def _router(self):
