@@ -1055,7 +1055,7 @@ class StageProgram:
         self.blocks = list(blocks)
         self.live_buffers = live_buffers
         self.dropout_seed = dropout_seed
-        self.dropout_mode: Tuple[bool, ...] = ()   # which blocks with dropout were in training mode when lowered
+        self.dropout_rates: Tuple[float, ...] = ()   # of the blocks that may drop, as the launch lists hold them
         self._rng: Dict[int, torch.Tensor] = {}
         self.device = device
         self.training = training

@@ -126,9 +126,8 @@ class PipelineStageBase:
             m for m in submodule.modules()
             if (isinstance(m, nn.modules.dropout._DropoutNd) and m.p > 0)
             or (isinstance(m, nn.MultiheadAttention) and m.dropout > 0)]
-        # blocks with a dropout of their own, which runs inside the launch lists while they are in training mode
-        self._dropout_blocks = [blk for blk in self._blocks or ()
-                                if isinstance(getattr(blk, "dropout", None), float) and blk.dropout > 0]
+        # blocks that may have a dropout of their own, which runs inside the launch lists while they are in training mode
+        self._dropout_blocks = [blk for blk in self._blocks or () if hasattr(blk, "live_dropout")]
         self._live_buffers = P.LiveBuffers(self._blocks or (), self.device)
         self._program: Optional[P.StageProgram] = None
         #: why this stage runs through torch autograd instead of HIP launch lists (None: it is native)
@@ -229,14 +228,15 @@ class PipelineStageBase:
             self._program.mbs.clear()
         return self._program
 
-    def _follow_dropout_mode(self, sp: P.StageProgram) -> None:
-        """A launch list holds its dropouts or not: it is lowered again for the mode its blocks are in now."""
-        mode = tuple(blk.training for blk in self._dropout_blocks)
-        if mode != sp.dropout_mode:
+    def _follow_dropout_rates(self, sp: P.StageProgram) -> None:
+        """A launch list holds its dropouts and their rates, or none: it is lowered again for the rates its blocks have
+        now (0 in eval mode)."""
+        rates = tuple(blk.live_dropout() for blk in self._dropout_blocks)
+        if rates != sp.dropout_rates:
             if self.has_backward and self.fwd_cache:
-                raise RuntimeError(f"{self.log_prefix} was switched between training and eval mode with microbatches "
-                                   "in flight")
-            sp.dropout_mode = mode
+                raise RuntimeError(f"{self.log_prefix} was switched between training and eval mode, or to another dropout "
+                                   "rate, with microbatches in flight")
+            sp.dropout_rates = rates
             sp.mbs.clear()
 
     def _dropout_seed(self) -> int:
@@ -371,7 +371,7 @@ class PipelineStageBase:
                 "autograd), or set the dropout probabilities to 0")
         sp = self._stage_program()
         if self._dropout_blocks:
-            self._follow_dropout_mode(sp)
+            self._follow_dropout_rates(sp)
         x, dx_target, patch = self._input_for(mb, args, kwargs)
         expected = self._exported_input_shape()
         if expected is not None and tuple(x.shape[1:]) != expected:

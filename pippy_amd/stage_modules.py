@@ -464,9 +464,8 @@ class TransformerLayer(NativeBlock):
                  dropout: float = 0.0):
         super().__init__()
         assert dim % n_heads == 0 and activation in ("gelu_tanh", "gelu_erf", "relu")
-        if not 0.0 <= dropout < 1.0:
-            raise ValueError(f"dropout must lie in [0, 1), not {dropout}")
         self.dropout = float(dropout)
+        self.live_dropout()
         self.dim, self.n_heads, self.ffn = dim, n_heads, ffn
         self.causal, self.pre_ln, self.activation = causal, pre_ln, activation
         self.ln_1 = nn.LayerNorm(dim, eps=eps, dtype=dtype)
@@ -496,10 +495,17 @@ class TransformerLayer(NativeBlock):
         o = F.scaled_dot_product_attention(q, k, v, is_causal=self.causal, scale=self.attn_scale)
         return self.attn.c_proj(o.transpose(1, 2).reshape(Bn, S, Cc))
 
+    def live_dropout(self) -> float:
+        """The rate that a step drops at now: ``dropout`` in training mode, else 0."""
+        if not 0.0 <= self.dropout < 1.0:
+            raise ValueError(f"dropout must lie in [0, 1), not {self.dropout}")
+        return float(self.dropout) if self.training else 0.0
+
     def _drop(self, branch, which):
         """Dropout of residual branch ``which`` (0: attention, 1: feed-forward).  The launch lists draw their masks
         from their own counter-based generator: the same distribution, other masks than torch's."""
-        return F.dropout(branch, self.dropout, self.training) if self.dropout > 0 else branch
+        rate = self.live_dropout()
+        return F.dropout(branch, rate, True) if rate > 0 else branch
 
     def forward(self, x):
         if self.pre_ln:
@@ -510,17 +516,18 @@ class TransformerLayer(NativeBlock):
 
     def _lower_branch(self, b, name, lin, h2d, resid):
         """Emits resid + dropout(lin(h)); returns it and the emitter of the branch's output gradient, dy -> d lin(h)."""
-        if not (self.dropout > 0 and self.training):
+        rate = self.live_dropout()
+        if rate == 0:
             y, _ = lower_linear(b, name, lin, h2d, epilogue=N.EPI_BIAS_RESIDUAL, aux_in=resid)
             return y, lambda dy2d: dy2d
         rng, site = b.dropout_site()
         branch, _ = lower_linear(b, name + ".branch", lin, h2d)
         y = b.act(name, tuple(branch.shape))
-        b.f(P.op_dropout(branch, y, rng, self.dropout, site, resid=resid))
+        b.f(P.op_dropout(branch, y, rng, rate, site, resid=resid))
 
         def backward(dy2d):
             d_branch = b.grad(name + ".d_branch", tuple(branch.shape))
-            b.i(P.op_dropout(dy2d, d_branch, rng, self.dropout, site))
+            b.i(P.op_dropout(dy2d, d_branch, rng, rate, site))
             return d_branch
 
         return y, backward

@@ -10,6 +10,7 @@ DEV = "cuda"
 K, E, L, M, S, VOCAB = 2, 12, 2, 2, 64, 128
 
 
+# ---- the balancing bias of a router ----------------------------------------------------------------------------
 def moe_model():
     from pippy_amd.configs import MoEDecoderLM
     torch.manual_seed(3)
@@ -145,3 +146,63 @@ def test_a_tensor_assigned_as_balancing_bias_stays_where_it_is_and_is_read_anew_
         selected_under(stages, [pushing(e), pushing(e + 1)])
         assert all(layer.block_sparse_moe.balance_bias is bias and bias.device.type == "cpu"
                    for layer, bias in zip(model.h, own))
+
+# ---- the dropout rate of a layer ------------------------------------------------------------------------------
+def dropout_pipeline(**options):
+    import pippy_amd as pp
+    from pippy_amd.configs import DecoderLM, equal_split_spec
+    torch.manual_seed(6)
+    model = DecoderLM(vocab=VOCAB, max_seq=S, dim=64, n_layers=L, n_heads=1, ffn=128, **options)
+    ids = torch.randint(0, VOCAB, (M, S))
+    pipe = pp.pipeline(model, M, (ids,), split_spec=equal_split_spec(L, 2))
+    stages = [pp.PipelineStage(pipe, i, DEV) for i in range(2)]
+    assert all(st.is_native for st in stages), [st.eager_reason for st in stages]
+    sched = pp.ScheduleGPipe(stages, M, loss_fn=pp.CrossEntropyLoss())
+    target = torch.randint(0, VOCAB, (M, S)).to(DEV)
+    ids = ids.to(DEV)
+
+    def step():
+        sched.zero_grad()
+        out = sched.step(ids, target=target, losses=[]).clone()
+        torch.cuda.synchronize()
+        return out, {n: p.main_grad.clone() for n, p in model.named_parameters()}
+
+    return model, stages, step
+
+
+def same(a, b):
+    return torch.equal(a[0], b[0]) and all(torch.equal(v, b[1][n]) for n, v in a[1].items())
+
+
+def test_a_dropout_rate_changed_between_steps_is_followed():
+    """A pipeline built at one rate and set to another gives what one built at that rate gives from the same state."""
+    def at(rate, offset):
+        model, stages, step = dropout_pipeline(dropout=rate)
+        if rate:
+            for st in stages:
+                for m in range(M):
+                    st._stage_program().rng_state(m)[1] += offset
+        return step()
+
+    model, stages, step = dropout_pipeline(dropout=0.0)
+    assert same(step(), at(0.0, 0))
+    for n, rate in enumerate((0.2, 0.5, 0.0, 0.1)):         # (a step without dropout does not move the state)
+        for layer in model.h:
+            layer.dropout = rate
+        assert same(step(), at(rate, n if rate != 0.1 else n - 1)), rate
+    for layer in model.h:
+        layer.dropout = 0                                   # an integer is a rate, too
+    assert same(step(), at(0.0, 0))
+
+
+@pytest.mark.parametrize("rate", [1.0, -0.1, float("nan")])
+def test_a_dropout_rate_out_of_range_is_refused(rate):
+    model, stages, step = dropout_pipeline(dropout=0.1)
+    step()
+    model.h[1].dropout = rate
+    with pytest.raises(RuntimeError, match="dropout"):
+        step()
+    model.h[1].dropout = 0.1
+    for st in stages:
+        st.clear_runtime_states()
+    step()
