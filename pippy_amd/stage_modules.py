@@ -521,12 +521,11 @@ class TransformerLayer(NativeBlock):
             y, _ = lower_linear(b, name, lin, h2d, epilogue=N.EPI_BIAS_RESIDUAL, aux_in=resid)
             return y, lambda dy2d: dy2d
         rng, site = b.dropout_site()
-        branch, _ = lower_linear(b, name + ".branch", lin, h2d)
-        y = b.act(name, tuple(branch.shape))
-        b.f(P.op_dropout(branch, y, rng, rate, site, resid=resid))
+        y, _ = lower_linear(b, name, lin, h2d)
+        b.f(P.op_dropout(y, y, rng, rate, site, resid=resid))    # in place: nothing reads lin(h) again
 
         def backward(dy2d):
-            d_branch = b.grad(name + ".d_branch", tuple(branch.shape))
+            d_branch = b.grad(name + ".d_branch", tuple(y.shape))
             b.i(P.op_dropout(dy2d, d_branch, rng, rate, site))
             return d_branch
 

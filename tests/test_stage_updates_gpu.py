@@ -206,3 +206,15 @@ def test_a_dropout_rate_out_of_range_is_refused(rate):
     for st in stages:
         st.clear_runtime_states()
     step()
+
+
+@pytest.mark.parametrize("pre_ln", [True, False])
+def test_dropout_keeps_no_activation_of_its_own(pre_ln):
+    """What a microbatch keeps for its backward is the same with dropout and without: the mask is formed again, and nothing
+    reads the branches in front of it."""
+    kept = []
+    for rate in (0.0, 0.2):
+        _, stages, step = dropout_pipeline(dropout=rate, pre_ln=pre_ln)
+        step()
+        kept.append([sorted((tuple(t.shape), t.dtype) for t in st.saved_activations(0).values()) for st in stages])
+    assert kept[0] == kept[1]
