@@ -353,8 +353,9 @@ int pp_moe_gate_bwd(const void* dout, int64_t ld_dout, const void* y, int64_t ld
  *   gate[t, k] = scale * s[idx_k] / (renorm ? sum_j s[idx_j] : 1)         (a sum of 0 gives gates of 0)
  * A logit of -infinity takes its expert out: it is not selected and counts in no sum; a token with fewer than
  * topk experts left has topk_idx -1 and gate 0 in its last slots, which the permutations drop (position -1).  A
- * NaN logit ranks behind every number; it makes the token's softmax weights NaN (renormalised ones only if it is
- * selected, since they are formed from the selected logits alone).
+ * NaN logit ranks behind every number, counts in no group's score and does not change the choices of the other
+ * experts; +infinity has all of the softmax for the selection (several share it).  Either makes the token's softmax
+ * weights NaN (renormalised ones only if it is selected, since they are formed from the selected logits alone).
  * Backward: the gradient of the logits from dgate (fp32 [T, topk]), or, with dgate null, from
  * dgate[t, k] = <dout[t, :], y[pos[t, k], :]> formed on the way (dout bf16 [T, C], y the bf16 expert rows, pos as
  * pp_moe_permute gives it; a negative position or index counts as no contribution).  The bias gets no gradient.

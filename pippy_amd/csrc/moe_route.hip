@@ -108,14 +108,14 @@ __device__ __forceinline__ float route_margin(float s_max, float c) {
 template <bool SIGMOID>
 __device__ __forceinline__ double route_score64(float x, float m, double sum) {
     if constexpr (SIGMOID) return 1.0 / (1.0 + exp(-(double)x));
-    else return exp((double)x - (double)m) / sum;
+    else return (x == m ? 1.0 : exp((double)x - (double)m)) / sum;
 }
 template <typename LT, int G>
 __device__ __forceinline__ double route_sum64(const RouteArgs& a, int64_t t, int li, float m) {
     double sum = 0.0;
     for (int e = li; e < a.E; e += G) {
         const float x = route_load<LT>(a.logits, t * a.ld + e);
-        if (x != -INFINITY) sum += exp((double)x - (double)m);
+        if (x == x && x != -INFINITY) sum += x == m ? 1.0 : exp((double)x - (double)m);
     }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -186,6 +186,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
     // scores of all experts in fp32, where anything needs them: the choices of a bias or of sums over groups, or
     // the sum of softmax weights that are not renormalised
     const bool top2 = a.n_group > 1 && a.group_top2;
+    // (a NaN enters neither the maximum nor the sum, only its own score; infinite logits share all of the softmax)
     float m = -INFINITY, sum = 1.f, s_max = 1.f;
     float s[V];
 #pragma unroll
@@ -202,11 +203,17 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
         sum = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            s[j] = x[j] == -INFINITY ? 0.f : expf(x[j] - m);
-            sum += s[j];
+            s[j] = x[j] == -INFINITY ? 0.f : x[j] == m ? 1.f : expf(x[j] - m);
+            sum += x[j] == x[j] ? s[j] : 0.f;
         }
         sum = route_fsum<G>(sum);
         s_max = 1.0f / sum;
+        if (!a.renorm) {  // softmax weights of a row with a NaN or an infinite logit are NaN
+            uint32_t lost = m == INFINITY;
+#pragma unroll
+            for (int j = 0; j < V; ++j) lost |= x[j] != x[j];
+            if (route_max<G>(lost)) sum = NAN;
+        }
         if (BIASED || top2) {
 #pragma unroll
             for (int j = 0; j < V; ++j) s[j] *= s_max;
@@ -492,6 +499,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
             if (top > 1) {
                 const float v = route_value(top);
                 from = route_key(v - route_margin<SIGMOID>(s_max, v));
+                from = from < 2 ? 2 : from;  // (a NaN is no candidate beside a number)
             }
         }
         uint32_t cand = 0;  // this lane's experts that may be the largest
