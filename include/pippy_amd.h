@@ -350,7 +350,8 @@ int pp_moe_gate_bwd(const void* dout, int64_t ld_dout, const void* y, int64_t ld
  *   stay open (ties: the lower group)
  *   topk_idx[t, :]: the topk largest choices of open groups, descending, ties to the lower expert; choices are
  *   compared in 64 bits (without a bias the logits themselves are compared)
- *   gate[t, k] = scale * s[idx_k] / (renorm ? sum_j s[idx_j] : 1)         (a sum of 0 gives gates of 0)
+ *   gate[t, k] = scale * s[idx_k] / (renorm ? sum_j s[idx_j] : 1)         (a sum that 64 bits hold as 0, of sigmoid
+ *   scores of logits below -709.7, gives gates of 0)
  * A logit of -infinity takes its expert out: it is not selected and counts in no sum; a token with fewer than
  * topk experts left has topk_idx -1 and gate 0 in its last slots, which the permutations drop (position -1).  A
  * NaN logit ranks behind every number, counts in no group's score and does not change the choices of the other

@@ -93,6 +93,16 @@ __device__ __forceinline__ float route_fsum(float v) {
     }));
 }
 
+// Sigmoid scores for the weights: e^-ref / (1 + e^-x), with both exponents at most 0.  Renormalised weights take them relative
+// to the largest selected logit where that is negative: fp32 holds no score below e^-103, but their ratios it does.
+__device__ __forceinline__ float route_sigmoid(float x, float ref) { return expf(fminf(x, 0.f) - ref) / (1.0f + expf(-fabsf(x))); }
+// The largest logit whose score 64 bits hold as 0 (e^-x overflows): selected logits that are all as low, as a mask writes
+// them, have a sum of 0 and weights of 0.
+constexpr float kRouteNoScore = -709.78271484375f;
+__device__ __forceinline__ float route_sigmoid_renorm(float x, float most) {
+    return most <= kRouteNoScore && x == x ? 0.f : route_sigmoid(x, fminf(most, 0.f));
+}
+
 // How far apart two choices formed in fp32 must be for their order to be certain.  A score is off by at most
 //   sigmoid: s (1 - s) (1.5 |x| 2^-24 + 2^-23) from the exponential (|x| s (1 - s) < 0.23), 3 s 2^-24 from the quotient:
 //            below 2^-21;
@@ -555,11 +565,11 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
         xs[q] = e[q] >= 0 ? route_load<LT>(a.logits, t * a.ld + e[q]) : -INFINITY;
         most = fmaxf(most, xs[q]);
     }
-    // renormalised softmax weights need no other expert: relative to the largest selected logit
-    if (!SIGMOID && a.renorm) most = route_fmax<G>(most);
+    // renormalised weights need no other expert: relative to the largest selected logit
+    if (a.renorm) most = route_fmax<G>(most);
 #pragma unroll
     for (int q = 0; q < kOwn; ++q) {
-        if (SIGMOID) w[q] = 1.0f / (1.0f + expf(-xs[q]));
+        if (SIGMOID) w[q] = a.renorm ? route_sigmoid_renorm(xs[q], most) : route_sigmoid(xs[q], 0.f);
         else w[q] = a.renorm ? expf(xs[q] - most) : expf(xs[q] - m) / sum;
         if (e[q] < 0) w[q] = 0.f;
         part += w[q];
@@ -580,7 +590,8 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
 //   d s[idx_k] = scale (dgate_k - sum_j g'_j dgate_j) / sum_j s[idx_j]   (renorm),   scale dgate_k   (otherwise)
 //   softmax: dx_e = s_e (ds_e - sum_j s_j ds_j);   sigmoid: dx_e = ds_e s_e (1 - s_e)
 // Renormalised softmax weights are a softmax over the selected logits alone, dx_k = scale g'_k (dgate_k - sum g' dgate),
-// and sigmoid scores do not mix: only softmax weights that are not renormalised read the whole row.
+// sigmoid ones have a factor (1 - s_k) besides (formed from the weights g', not from ds, whose quotient overflows where all
+// scores are small), and sigmoid scores do not mix: only softmax weights that are not renormalised read the whole row.
 // dgate_k is given, or <dout[t], y[pos(t, k)]> over the expert rows.
 //
 // One wave per token; lane k < K holds slot k.  Bound by the expert rows: per chunk of 512 columns the loads of the
@@ -661,12 +672,10 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
     float dot = 0.f;
     if (SIGMOID || a.renorm) {
         float w;
-        if constexpr (SIGMOID) {
-            w = e >= 0 ? 1.0f / (1.0f + expf(-xe)) : 0.f;
-        } else {
-            const float most = wave_max(xe);
-            w = e >= 0 ? expf(xe - most) : 0.f;
-        }
+        const float most = a.renorm ? wave_max(xe) : 0.f;
+        if constexpr (SIGMOID) w = route_sigmoid_renorm(xe, most);
+        else w = expf(xe - most);
+        if (e < 0) w = 0.f;
         float ds = a.scale * dg;
         if (a.renorm) {
             // differences against the first slot's gradient (the weights sum to one): a token with a single expert
@@ -674,7 +683,8 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
             const float total = wave_sum(w), g = total == 0.f ? 0.f : w / total;
             const float rel = dg - __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(dg)));
             ds = a.scale * (rel - wave_sum(e >= 0 ? g * rel : 0.f));
-            dx = SIGMOID ? (total == 0.f ? 0.f : ds / total * w * (1.0f - w)) : ds * g;
+            dx = ds * g;
+            if (SIGMOID) dx *= 1.0f - route_sigmoid(xe, 0.f);
         } else {
             dx = ds * w * (1.0f - w);
         }

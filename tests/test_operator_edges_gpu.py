@@ -90,3 +90,52 @@ def test_routing_ranks_a_nan_behind_every_number(scoring, biased, E, k, groups, 
             assert bool(gate.cpu()[(want >= 0) & bad].isnan().all())
         else:
             assert bool(gate.cpu()[hit].isnan().all())
+
+
+@pytest.mark.parametrize("base", [-60.0, -82.0, -85.5, -88.5, -95.0, -300.0, -700.0])
+@pytest.mark.parametrize("k", [1, 3, 8])
+def test_renormalised_sigmoid_weights_of_small_scores(base, k):
+    """Scores far below what fp32 holds still have ratios.  The weights are quotients of exponentials of differences up to
+    4: 4 x 2^-24 from the difference, 2^-23 from every exponential, 2^-22 from sums and quotients, 2^-20 in all; a gradient is two
+    such products, and the fp32 sum of g dgate before it (K terms, 2^-21 of its absolute values)."""
+    N = native()
+    T, E = 40, 32
+    g = torch.Generator().manual_seed(k)
+    x = base - 4 * torch.rand(T, E, generator=g)
+    dgate = torch.randn(T, k, generator=g) * 1000
+    idx = torch.empty(T, k, dtype=torch.int32, device=DEV)
+    gate = torch.empty(T, k, device=DEV)
+    N.moe_route(x.to(DEV), idx, gate, scoring="sigmoid", scale=1.5)
+    xr = x.double().requires_grad_(True)
+    want_idx, want = O.moe_route(xr, k, scoring="sigmoid", scale=1.5)
+    assert torch.equal(idx.cpu().long(), want_idx)
+    want = want.detach()
+    assert float(want.sum(-1).min()) > 1.49
+    within(gate, want, 2.0 ** -20 * want, "gate")
+    dl = torch.empty(T, E, device=DEV)
+    N.moe_route_bwd(x.to(DEV), idx, dl, dgate=dgate.to(DEV), scoring="sigmoid", scale=1.5)
+    # d gate_k / d x_k = gate_k (1 - g_k) (1 - s_k), formed without the quotient s / sum s that autograd would take
+    s1, w = torch.sigmoid(-x.double()).gather(1, want_idx), want / 1.5
+    d = dgate.double()
+    dx = 1.5 * (d - (w * d).sum(-1, keepdim=True)) * w * s1
+    size = 1.5 * (d.abs() + (w * d.abs()).sum(-1, keepdim=True)) * w * s1
+    wanted = torch.zeros(T, E, dtype=torch.float64).scatter(1, want_idx, dx)
+    bound = torch.zeros(T, E, dtype=torch.float64).scatter(1, want_idx, 2.0 ** -18 * size)
+    within(dl, wanted, bound, "dlogits")
+
+
+def test_scores_that_64_bits_hold_as_zero_give_no_weight():
+    """Logits at the lowest value of their type, as masks are written: the sum of the scores is 0, the weights are 0."""
+    N = native()
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.full((3, 8), torch.finfo(dtype).min, dtype=dtype)
+        x[1, 2] = -750.0
+        x[2, 5] = -2.0
+        idx = torch.empty(3, 2, dtype=torch.int32, device=DEV)
+        gate = torch.empty(3, 2, device=DEV)
+        N.moe_route(x.to(DEV), idx, gate, scoring="sigmoid")
+        want_idx, want = O.moe_route(x.double(), 2, scoring="sigmoid")
+        assert torch.equal(idx.cpu().long(), want_idx) and torch.equal(gate.cpu().double(), want)
+        dl = torch.full((3, 8), 9.0, dtype=dtype, device=DEV)
+        N.moe_route_bwd(x.to(DEV), idx, dl, dgate=torch.tensor([[1.0, 2.0]] * 3, device=DEV), scoring="sigmoid")
+        assert bool((dl == 0).all())
