@@ -673,7 +673,7 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
     if (SIGMOID || a.renorm) {
         float w;
         const float most = a.renorm ? wave_max(xe) : 0.f;
-        if constexpr (SIGMOID) w = route_sigmoid_renorm(xe, most);
+        if constexpr (SIGMOID) w = a.renorm ? route_sigmoid_renorm(xe, most) : route_sigmoid(xe, 0.f);
         else w = expf(xe - most);
         if (e < 0) w = 0.f;
         float ds = a.scale * dg;
@@ -684,9 +684,9 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
             const float rel = dg - __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(dg)));
             ds = a.scale * (rel - wave_sum(e >= 0 ? g * rel : 0.f));
             dx = ds * g;
-            if (SIGMOID) dx *= 1.0f - route_sigmoid(xe, 0.f);
+            if (SIGMOID) dx *= route_sigmoid(-xe, 0.f);  // 1 - s, which a subtraction would lose for large logits
         } else {
-            dx = ds * w * (1.0f - w);
+            dx = ds * w * route_sigmoid(-xe, 0.f);
         }
         if (e < 0) dx = 0.f;
     } else {

@@ -139,3 +139,29 @@ def test_scores_that_64_bits_hold_as_zero_give_no_weight():
         dl = torch.full((3, 8), 9.0, dtype=dtype, device=DEV)
         N.moe_route_bwd(x.to(DEV), idx, dl, dgate=torch.tensor([[1.0, 2.0]] * 3, device=DEV), scoring="sigmoid")
         assert bool((dl == 0).all())
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+def test_sigmoid_gradient_of_large_logits(renorm):
+    """1 - s is formed as the sigmoid of -x, not by subtraction from 1.  Relative errors: 2^-23 each from the exponential, the sum and
+    the quotient of s and of 1 - s, 2^-20 with the sums over the slots."""
+    N = native()
+    T, E, k = 50, 16, 3
+    g = torch.Generator().manual_seed(5)
+    x = torch.rand(T, E, generator=g) * 40 + torch.linspace(-20, 40, T)[:, None]
+    dgate = torch.randn(T, k, generator=g)
+    idx, _ = O.moe_route(x.double(), k, scoring="sigmoid")
+    s = torch.sigmoid(x.double()).gather(1, idx)
+    rest = torch.sigmoid(-x.double()).gather(1, idx)
+    d = dgate.double()
+    if renorm:
+        w = s / s.sum(-1, keepdim=True)
+        dx = (d - (w * d).sum(-1, keepdim=True)) * w * rest
+        size = (d.abs() + (w * d.abs()).sum(-1, keepdim=True)) * w * rest
+    else:
+        dx = d * s * rest
+        size = dx.abs()
+    dl = torch.empty(T, E, device=DEV)
+    N.moe_route_bwd(x.to(DEV), idx.int().to(DEV), dl, dgate=dgate.to(DEV), scoring="sigmoid", renorm=renorm)
+    zero = torch.zeros(T, E, dtype=torch.float64)
+    within(dl, zero.scatter(1, idx, dx), zero.scatter(1, idx, 2.0 ** -20 * size), "dlogits")
