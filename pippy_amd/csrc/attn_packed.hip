@@ -495,9 +495,17 @@ __device__ __forceinline__ float packed_delta(const uint16_t* qp, const uint16_t
 }
 
 // A work-group owns 64 query rows (2 groups of 32 queries x 2 halves of every key block) and hands the dK / dV
-// kernel the row sums D = sum_j P dP; its own dS uses them where they are known in time, in a block with one block of
-// keys, and delta elsewhere.  Bound like the forward's form of 64 rows: [4096 rows in 11 documents, 12 heads of
-// 64], causal: 19 us.
+// kernel the row sums D = sum_j P dP.
+//
+// dS = P (dP - D), but D is known only behind the loop.  The loop takes delta = rowsum(dO O) of the stored output for it, which
+// the rounding of the output keeps from D by r = D - delta, and so leaves a surplus of r P k_j for every key: r times the
+// weighted mean of the keys, which dwarfs dQ where weights are nearly even and keys and values have common parts (with
+// parts of 16 standard deviations, 2000 keys: an error of 7 times dQ causal, 20 without a mask).  P K is therefore summed beside
+// dS K and r P K taken off at the end.  That is a product more per block, of fragments that are there: 4096 rows in 11
+// documents, 12 heads of 64: whole backward 40 -> 42 us; 8192 rows in 5 documents, 32 / 8 heads of 128: 548 -> 638 us, where its
+// registers also end a form of 128 rows per work-group (with it 1118 us with spills, 671 with one wave per SIMD).
+// For head dimension 128 the rows of dO lie in LDS for want of registers (in registers 668 us).
+// In a block with one block of keys D is formed before dS.  Bound like the forward's form of 64 rows.
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -528,20 +536,27 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
     const uint16_t* op = a.o + row * a.so + (int64_t)w.h * D;
     bf16x8_t qf[KS], dof[KS];
     float delta_q = packed_delta<KS>(qp, dop, op, lh, qf, dof);
+    uint16_t* const Ol = lds + NS * kStage;
+    if constexpr (D == 128) {
+        PackedTileLoader<DS> lo;
+        lo.init(a.d_o + w.row0 * a.sdo + (int64_t)w.h * D, a.sdo, w.len, wave, lane);
+        lo.load(Ol, q0, wave);
+    }
     const float lse_q = a.lse[(int64_t)w.h * a.T + row] * kLog2e;
-    // The sum of P dP over the keys equals delta in exact arithmetic and is the one under which the rows of dS
-    // sum to zero; it is complete only behind the loop and is what the dK / dV kernel gets.
-    float d_sum = 0.f;
+    float d_sum = 0.f;  // D
 #pragma unroll
     for (int t = 0; t < NS - 1; ++t)
         if (t < n_blocks) issue(t, t);
     const float c = a.scale * kLog2e;
 
-    f32x16_t dqacc[DT];
+    f32x16_t dqacc[DT], pkacc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dqacc[t][e] = 0.f;
+        for (int e = 0; e < 16; ++e) {
+            dqacc[t][e] = 0.f;
+            pkacc[t][e] = 0.f;
+        }
 
     // P and dP of a block; P dP goes into the sum
     auto weights = [&](auto masked_c, const uint16_t* Ks, int j, float (&dsv)[16], f32x16_t& dpacc)
@@ -558,7 +573,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
             const bf16x8_t kfr = read_row_frag<swz_packed>(Ks + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             const bf16x8_t vfr = read_row_frag<swz_packed>(Vs + (ks / 4) * kTile, 32 * half + l32, 2 * (ks % 4) + lh);
             sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr, qf[ks], sacc, 0, 0, 0);
-            dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr, dof[ks], dpacc, 0, 0, 0);
+            bf16x8_t of;
+            if constexpr (D == 128) of = read_row_frag<swz_packed>(Ol + (ks / 4) * kTile, 32 * grp + l32, 2 * (ks % 4) + lh);
+            else of = dof[ks];
+            dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr, of, dpacc, 0, 0, 0);
         }
 #pragma unroll
         for (int v = 0; v < 16; ++v) dsv[v] = __builtin_amdgcn_exp2f(fmaf(sacc[v], c, -lse_q));
@@ -575,6 +593,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         float dsv[16];
         f32x16_t dpacc;
         weights(masked_c, Ks, j, dsv, dpacc);
+        const bf16x8_t pb[2] = {pack8(dsv), pack8(dsv + 8)};
 #pragma unroll
         for (int v = 0; v < 16; ++v) dsv[v] *= dpacc[v] - delta_q;
 #pragma unroll
@@ -584,6 +603,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
             for (int dt = 0; dt < DT; ++dt) {
                 const bf16x8_t ktf = read_col_frag<swz_packed>(Ks + (dt / 2) * kTile, 32 * half + 16 * gp, 32 * (dt % 2), lane);
                 dqacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktf, dsb, dqacc[dt], 0, 0, 0);
+                pkacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktf, pb[gp], pkacc[dt], 0, 0, 0);
             }
         }
     };
@@ -621,20 +641,27 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         if (kt0 < w.len && (!CAUSAL || kt0 <= qw0 + 31)) step(std::true_type{}, Ks, j);
     }
     d_sum += __shfl_xor(d_sum, 32, 64);
-    // add the sums of the two halves: [grp][16 DT + 1 values][64 lanes] floats
+    // add the sums of the two halves, first the row sums, then [grp][16 DT values][64 lanes] floats
+    float* rows = reinterpret_cast<float*>(lds) + 2 * 16 * DT * 64;
+    float* xs = reinterpret_cast<float*>(lds) + grp * (16 * DT * 64) + lane;
     wait_lds();
     __syncthreads();
-    float* xs = reinterpret_cast<float*>(lds) + grp * ((16 * DT + 1) * 64) + lane;
+    rows[wave * 64 + lane] = d_sum;
+    __syncthreads();
+    d_sum += rows[(wave ^ 2) * 64 + lane];
+    const float r = d_sum - delta_q;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dqacc[dt][e] = fmaf(-r, pkacc[dt][e], dqacc[dt][e]);
     if (half == 1) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) xs[(16 * dt + e) * 64] = dqacc[dt][e];
-        xs[16 * DT * 64] = d_sum;
     }
     __syncthreads();
     if (half == 1 || qi >= w.len) return;
-    d_sum += xs[16 * DT * 64];
     if (lh == 0) a.delta[(int64_t)w.h * a.T + row] = d_sum;
     uint16_t* dqp = a.dq + row * a.sdq + (int64_t)w.h * D;
 #pragma unroll
@@ -646,136 +673,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
             for (int e = 0; e < 4; ++e) s[e] = (dqacc[dt][4 * g + e] + xs[(16 * dt + 4 * g + e) * 64]) * a.scale;
             const int d = 32 * dt + 8 * g + 4 * lh;
             *reinterpret_cast<uint2*>(dqp + d) = make_uint2(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]));
-        }
-}
-
-// The form for long sequences: 128 query rows, 32 per wave, every wave over all keys (see the forward).  Three
-// products per pair of blocks: 213 us for causal [8192 rows in 5 documents, 32 query and 8 key / value heads of 128].
-template <int D, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void attn_packed_bwd_dq128_kernel(const PackedArgs a) {
-    constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
-    constexpr int kOperand = DS * kTile, kStage = 2 * kOperand;
-    uint16_t* const lds = attn_lds;
-
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l32 = lane & 31, lh = lane >> 5;
-    PackedBlock w;
-    if (!packed_block_of<CAUSAL, true>(a, a.H, &w)) return;
-    const int q0 = w.j * 128, qw0 = q0 + 32 * wave, qi = qw0 + l32;
-    const int hk = w.h / a.G;
-
-    PackedTileLoader<DS> lk, lv;
-    lk.init(a.k + w.row0 * a.sk + (int64_t)hk * D, a.sk, w.len, wave, lane);
-    lv.init(a.v + w.row0 * a.sv + (int64_t)hk * D, a.sv, w.len, wave, lane);
-    const int n_keys = CAUSAL && q0 + 128 < w.len ? q0 + 128 : w.len;
-    const int n_blocks = (n_keys + 63) / 64;
-    auto issue = [&](int stage, int j) {
-        lk.load(lds + stage * kStage, j * 64, wave);
-        lv.load(lds + stage * kStage + kOperand, j * 64, wave);
-    };
-
-    const int qr = qi < w.len ? qi : w.len - 1;
-    const int64_t row = w.row0 + qr;
-    const uint16_t* qp = a.q + row * a.sq + (int64_t)w.h * D;
-    const uint16_t* dop = a.d_o + row * a.sdo + (int64_t)w.h * D;
-    const uint16_t* op = a.o + row * a.so + (int64_t)w.h * D;
-    bf16x8_t qf[KS], dof[KS];
-    const float delta_q = packed_delta<KS>(qp, dop, op, lh, qf, dof);
-    const float lse_q = a.lse[(int64_t)w.h * a.T + row] * kLog2e;
-    float d_sum = 0.f;
-#pragma unroll
-    for (int t = 0; t < NS - 1; ++t)
-        if (t < n_blocks) issue(t, t);
-    const float c = a.scale * kLog2e;
-    const int seen = CAUSAL && qw0 + 32 < w.len ? qw0 + 32 : w.len;
-
-    f32x16_t dqacc[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dqacc[t][e] = 0.f;
-
-    auto step = [&](auto n_c, auto masked_c, const uint16_t* Ks, const uint16_t* Vs, int kr, int kt0)
-        __attribute__((always_inline)) {
-        constexpr int N = decltype(n_c)::value;
-        f32x16_t s[N], dp[N];
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[t][e] = 0.f;
-                dp[t][e] = 0.f;
-            }
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const bf16x8_t kfr = read_row_frag<swz_packed>(Ks + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
-                const bf16x8_t vfr = read_row_frag<swz_packed>(Vs + (ks / 4) * kTile, kr + 32 * t + l32, 2 * (ks % 4) + lh);
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr, qf[ks], s[t], 0, 0, 0);
-                dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr, dof[ks], dp[t], 0, 0, 0);
-            }
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[t][v] = __builtin_amdgcn_exp2f(fmaf(s[t][v], c, -lse_q));
-            if constexpr (decltype(masked_c)::value) {
-                const int lim = (CAUSAL ? qr : w.len - 1) - kt0 - 4 * lh;
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (32 * t + 8 * (v >> 2) + (v & 3) > lim) s[t][v] = 0.f;
-            }
-#pragma unroll
-            for (int v = 0; v < 16; ++v) d_sum = fmaf(s[t][v], dp[t][v], d_sum);
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[t][v] *= dp[t][v] - delta_q;
-#pragma unroll
-            for (int gp = 0; gp < 2; ++gp) {
-                float ds[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ds[e] = s[t][8 * gp + e];
-                const bf16x8_t dsb = pack8(ds);
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    const bf16x8_t ktf = read_col_frag<swz_packed>(Ks + (dt / 2) * kTile, kr + 32 * t + 16 * gp, 32 * (dt % 2), lane);
-                    dqacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ktf, dsb, dqacc[dt], 0, 0, 0);
-                }
-            }
-        }
-    };
-    const int n_whole = (CAUSAL && q0 < w.len ? q0 : w.len) / 64;
-    int j = 0;
-    for (; j + NS <= n_whole; j += NS)
-        static_for<NS>([&](auto stage_c) __attribute__((always_inline)) {
-            constexpr int stage = decltype(stage_c)::value;
-            await_block<4 * DS, NS>(j + stage, n_blocks);
-            if (j + stage + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + stage + NS - 1);
-            step(std::integral_constant<int, 2>{}, std::false_type{}, lds + stage * kStage, lds + stage * kStage + kOperand,
-                 0, (j + stage) * 64);
-        });
-    for (int stage = 0; j < n_blocks; ++j) {
-        await_block<4 * DS, NS>(j, n_blocks);
-        if (j + NS - 1 < n_blocks) issue(stage == 0 ? NS - 1 : stage - 1, j + NS - 1);
-        for (int t = 0; t < 2; ++t)
-            if (j * 64 + 32 * t < seen)
-                step(std::integral_constant<int, 1>{}, std::true_type{}, lds + stage * kStage,
-                     lds + stage * kStage + kOperand, 32 * t, j * 64 + 32 * t);
-        stage = stage + 1 == NS ? 0 : stage + 1;
-    }
-    d_sum += __shfl_xor(d_sum, 32, 64);
-    if (qi >= w.len) return;
-    if (lh == 0) a.delta[(int64_t)w.h * a.T + row] = d_sum;
-    uint16_t* dqp = a.dq + row * a.sdq + (int64_t)w.h * D;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = dqacc[dt][4 * g + e] * a.scale;
-            const int d = 32 * dt + 8 * g + 4 * lh;
-            *reinterpret_cast<uint2*>(dqp + d) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
         }
 }
 
@@ -1226,13 +1123,13 @@ static int packed_launch(const char* name, int threads, int64_t grid, size_t lds
     return check_launch(name);
 }
 
-// 128-row forms where the launch has at least as many blocks of 128 rows as the CUs hold work-groups at once (3 of
-// head dimension 64, 2 of 128; the sequences' last, partly filled blocks are left out of the count).  With fewer,
-// half as many work-groups leave CUs idle and the last one takes twice as long.  Forward, us, 64 rows | 128 rows:
+// The forward's form of 128 rows (for dK / dV 128 keys, below) where the launch has at least as many blocks of 128 as the
+// CUs hold work-groups at once (3 of head dimension 64, 2 of 128; the sequences' last, partly filled blocks are left
+// out of the count).  With fewer, half as many work-groups leave CUs idle and the last one takes twice as long.  Forward,
+// us, 64 rows | 128 rows:
 //   D = 64:  [16 heads] T = 2048: 23.7 | 27.6, 4096: 50.6 | 57.4; [12 heads] T = 8192: 150 | 129; [16] T = 16384 in 16
 //            sequences: 89.6 | 74.4, in 256: 42.8 | 39.1
 //   D = 128: [32 heads] T = 1024: 20.7 | 24.3, 2048: 50.6 | 49.7, 4096: 169 | 141, 16384 in 3 sequences: 1070 | 870
-// The backward's dQ takes it for D = 128 only (T = 16384, 16 heads of 64: 290 us against 306 for the whole backward).
 static bool packed_wide(const pp_attn_packed_desc* d, int64_t heads) {
     return d->T / 128 * heads >= (d->D == 64 ? 3 : 2) * 256;
 }
@@ -1251,6 +1148,7 @@ static int packed_fwd(const pp_attn_packed_desc* d, hipStream_t st) {
 template <int D, bool CAUSAL>
 static int packed_bwd(const pp_attn_packed_desc* d, hipStream_t st) {
     const PackedArgs a = packed_args(d);
+    constexpr int DS = D / 64;
     const int64_t blocks64 = plan_blocks64(d->T, d->n_seq), blocks128 = plan_blocks128(d->T, d->n_seq);
     // the dQ kernel goes first: it leaves the row sums that the dK / dV kernel reads
     const size_t lds = packed_lds_bytes(D);
@@ -1261,11 +1159,8 @@ static int packed_bwd(const pp_attn_packed_desc* d, hipStream_t st) {
         return packed_launch<attn_packed_bwd_dkv_kernel<CAUSAL>>("attn_packed_bwd_dkv_kernel", 256, blocks64 * d->Hkv,
                                                                  attn_stages(D) * (2 * kTile * 2 + 512), st, a);
     } else {
-        const int rc = packed_wide(d, d->H)
-                           ? packed_launch<attn_packed_bwd_dq128_kernel<D, CAUSAL>>("attn_packed_bwd_dq128_kernel", 256,
-                                                                                    blocks128 * d->H, lds, st, a)
-                           : packed_launch<attn_packed_bwd_dq_kernel<D, CAUSAL>>("attn_packed_bwd_dq_kernel", 256,
-                                                                                 blocks64 * d->H, lds, st, a);
+        const int rc = packed_launch<attn_packed_bwd_dq_kernel<D, CAUSAL>>("attn_packed_bwd_dq_kernel", 256, blocks64 * d->H,
+                                                                           lds + DS * kTile * 2, st, a);
         if (rc) return rc;
         // Whole backward, us, 64 | 128 keys per work-group: [32 query, 8 key / value heads] T = 2048: 187 | 262, 4096: 483 |
         // 599, 8192: 1794 | 1721, 16384 in 16 sequences: 649 | 594; [32, 32] T = 1024: 61.5 | 63.7, 2048: 166 | 147

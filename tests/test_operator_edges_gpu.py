@@ -165,3 +165,43 @@ def test_sigmoid_gradient_of_large_logits(renorm):
     N.moe_route_bwd(x.to(DEV), idx.int().to(DEV), dl, dgate=dgate.to(DEV), scoring="sigmoid", renorm=renorm)
     zero = torch.zeros(T, E, dtype=torch.float64)
     within(dl, zero.scatter(1, idx, dx), zero.scatter(1, idx, 2.0 ** -20 * size), "dlogits")
+
+
+@pytest.mark.parametrize("D,H,Hkv,cu", [(64, 2, 2, [0, 70, 326, 590]), (128, 4, 1, [0, 70, 326, 590]),
+                                        (64, 32, 32, [0, 2000, 2100]), (128, 32, 8, [0, 2000, 2100])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_query_gradient_under_nearly_uniform_attention_with_a_common_part(D, H, Hkv, cu, causal):
+    """Keys and values that share a large part: the gradient of a query is a small difference.  The common part of the keys
+    meets the sum of a row of dS, which is zero, so only the rounding of the terms of dS (2^-8 of each), fp32 noise of the
+    products (2^-16 of P |dP| and of its row's sum) and the result's own rounding may reach dQ.  The error of the stored
+    output, (2^-8 + 2^-8) P |V|, which is large beside dS, may not, but for products with a second rounding: that of dS, which
+    holds it, and that of P in its correction, 4 x 2^-16 |dO| P |V| together."""
+    N = native()
+    T = cu[-1]
+    g = torch.Generator().manual_seed(D + H + T)
+    q = (torch.randn(T, H, D, generator=g) * 0.05).to(torch.bfloat16)
+    common = torch.randn(2, 1, Hkv, D, generator=g) * 8
+    k, v = (torch.randn(2, T, Hkv, D, generator=g) * 0.5 + common).to(torch.bfloat16).unbind(0)
+    do = (torch.randn(T, H, D, generator=g) * 0.1).to(torch.bfloat16)
+    qd, kd, vd, dod = (t.to(DEV) for t in (q, k, v, do))
+    o, dq, dk, dv = torch.empty_like(qd), torch.empty_like(qd), torch.empty_like(kd), torch.empty_like(vd)
+    lse, delta = (torch.empty(H, T, device=DEV) for _ in range(2))
+    plan = N.attn_packed_plan(torch.tensor(cu, dtype=torch.int32, device=DEV), T)
+    N.attn_packed_fwd(qd, kd, vd, o, lse, plan, causal=causal)
+    N.attn_packed_bwd(qd, kd, vd, o, lse, dod, dq, dk, dv, delta, plan, causal=causal)
+    scale = D ** -0.5
+    for a, b in zip(cu[:-1], cu[1:]):
+        for h in range(0, H, max(1, H // 2)):
+            Q, dO = q[a:b, h].double(), do[a:b, h].double()
+            K, V = k[a:b, h * Hkv // H].double(), v[a:b, h * Hkv // H].double()
+            S = Q @ K.T * scale
+            if causal:
+                S = S.masked_fill(torch.ones(b - a, b - a, dtype=torch.bool).triu(1), float("-inf"))
+            P = torch.softmax(S, -1)
+            dP = dO @ V.T
+            dS = P * (dP - (P * dP).sum(-1, keepdim=True))
+            want = dS @ K * scale
+            noise = P * (dP.abs() + (P * dP.abs()).sum(-1, keepdim=True))
+            stored = P * (dO.abs() * (P @ V.abs())).sum(-1, keepdim=True)
+            bound = scale * (U * dS.abs() + 2.0 ** -16 * noise + 2.0 ** -14 * stored) @ K.abs() + U * want.abs()
+            within(dq[a:b, h], want, 1.02 * bound + 1e-30, "dq")
