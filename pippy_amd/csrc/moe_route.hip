@@ -741,8 +741,10 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
 // expert; its rank is the wave's count so far plus the members in front of it, and the first member counts for all.
 // Up to 4096 slots are one launch of one work-group.  More are two: the counts of every work-group, then every
 // work-group adds up the counts of all and of those in front of it and places its slots.  More rounds mean fewer
-// work-groups and fewer counts to read but longer chains; us for 1, 2, 4, 8 rounds, 256 experts: 32768 slots 8.0,
-// 8.8, 14.1, 20.3; 262144: 15.1, 12.8, 14.5, 20.9; 1048576: 68, 30, 23, 26; 4194304: 918, 262, 99, 74.
+// work-groups and fewer counts to read but longer chains; us for 1, 2, 4, 8 rounds, 256 experts: 65536 slots 8.8, 9.4, 12.8,
+// 21.4; 131072: 10.7, 10.4, 13.2, 20.0; 262144: 15.0, 12.8, 14.5, 20.7; 393216: 21.0, 15.1, 15.9, 21.6; 524288: 25.2, 17.6, 17.3,
+// 22.5; 1048576: 68, 30, 23, 26; 1310720: 115, 52, 32, 28 (64 experts: 65536 9.3, 9.3; 524288: 20.0, 14.4, 14.5; 1048576: 54, 24,
+// 19, 22).
 constexpr int kPermMaxE = 1024;
 constexpr int kPermThreads = 1024;
 constexpr int kPermWaves = kPermThreads / 64;
@@ -860,10 +862,10 @@ __global__ __launch_bounds__(kPermThreads) void moe_permute_place_kernel(const i
     }
 }
 
-// At most 64 R work-groups of R rounds (8: any number of them).
+// The rounds that measured fastest (above).
 static int perm_rounds(int64_t n) {
     if (n <= kPermOneLaunch) return 4;
-    return n <= 64 * 1024 ? 1 : n <= 4 * 64 * 1024 ? 2 : n <= 16 * 64 * 1024 ? 4 : 8;
+    return n <= 1 << 16 ? 1 : n <= 1 << 19 ? 2 : n <= 1 << 20 ? 4 : 8;
 }
 static int64_t perm_groups(int64_t n) {
     const int64_t slots = (int64_t)perm_rounds(n) * kPermThreads;

@@ -205,3 +205,21 @@ def test_query_gradient_under_nearly_uniform_attention_with_a_common_part(D, H, 
             stored = P * (dO.abs() * (P @ V.abs())).sum(-1, keepdim=True)
             bound = scale * (U * dS.abs() + 2.0 ** -16 * noise + 2.0 ** -14 * stored) @ K.abs() + U * want.abs()
             within(dq[a:b, h], want, 1.02 * bound + 1e-30, "dq")
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 65536, 65537, 300000, 524288, 524289, 1048576, 1048577])
+@pytest.mark.parametrize("E", [2, 250])
+def test_permutation_on_either_side_of_its_borders(n, E):
+    """Numbers of slots from which on a work-group takes more of them."""
+    N = native()
+    slots = torch.randint(-1, E, (n,), generator=torch.Generator().manual_seed(n), dtype=torch.int32)
+    kept = slots >= 0
+    seg = torch.full((E + 1,), -7, dtype=torch.int32, device=DEV)
+    row_src, pos = (torch.full((n,), -7, dtype=torch.int32, device=DEV) for _ in range(2))
+    ws = torch.full((N.moe_permute_workspace(n, E),), -9, dtype=torch.int32, device=DEV)
+    N.moe_permute_ws(slots.to(DEV), E, seg, row_src, pos, ws)
+    order = torch.sort(torch.where(kept, slots, torch.full_like(slots, E)), stable=True).indices[:int(kept.sum())]
+    counts = torch.bincount(slots[kept], minlength=E)
+    assert seg.tolist() == [0] + counts.cumsum(0).tolist()
+    assert torch.equal(row_src[:len(order)].cpu().long(), order) and bool((row_src[len(order):] == -7).all())
+    assert torch.equal(pos.cpu()[order].long(), torch.arange(len(order))) and bool((pos.cpu()[~kept] == -1).all())
