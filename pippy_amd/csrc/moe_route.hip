@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
     // scores of all experts in fp32, where anything needs them: the choices of a bias or of sums over groups, or
     // the sum of softmax weights that are not renormalised
     const bool top2 = a.n_group > 1 && a.group_top2;
-    // (a NaN enters neither the maximum nor the sum, only its own score; infinite logits share all of the softmax)
+    // (a NaN enters neither the maximum nor the sum of the choices, only its own; infinite logits share all of the softmax)
     float m = -INFINITY, sum = 1.f, s_max = 1.f;
     float s[V];
 #pragma unroll
@@ -213,17 +213,23 @@ __global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
         sum = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            s[j] = x[j] == -INFINITY ? 0.f : x[j] == m ? 1.f : expf(x[j] - m);
-            sum += x[j] == x[j] ? s[j] : 0.f;
+            s[j] = x[j] == -INFINITY ? 0.f : expf(x[j] - m);
+            sum += s[j];
         }
         sum = route_fsum<G>(sum);
-        s_max = 1.0f / sum;
-        if (!a.renorm) {  // softmax weights of a row with a NaN or an infinite logit are NaN
-            uint32_t lost = m == INFINITY;
+        const bool lost = sum != sum;  // the row has a NaN or an infinite logit
+        if (__any(lost)) {
+            float known = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) lost |= x[j] != x[j];
-            if (route_max<G>(lost)) sum = NAN;
+            for (int j = 0; j < V; ++j) {
+                if (lost) s[j] = x[j] == -INFINITY ? 0.f : x[j] == m ? 1.f : expf(x[j] - m);
+                known += x[j] == x[j] ? s[j] : 0.f;
+            }
+            known = route_fsum<G>(known);
+            if (lost) sum = known;
         }
+        s_max = 1.0f / sum;
+        if (lost && !a.renorm) sum = NAN;  // such a row's softmax weights
         if (BIASED || top2) {
 #pragma unroll
             for (int j = 0; j < V; ++j) s[j] *= s_max;
