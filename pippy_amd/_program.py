@@ -1018,32 +1018,37 @@ class LiveBuffers:
     """Buffers of a stage's modules that its launch lists read by address and a training loop updates between steps (a
     router's balancing bias).
 
-    Every buffer has one storage on the device for the life of the stage.  The tensor that the module holds when the stage
-    is built moves into it (the tensor object stays, as parameters stay when they move into the arena), so an update in
-    place through any reference to it is what the next kernel reads.  Whatever the module holds in its place later (an
-    assignment, ``load_state_dict(assign=True)``, ``module.to``) is copied into the storage at the beginning of every step."""
+    The lists read a copy of their own, which is made anew from the module at the beginning of every step: whatever was
+    done between two steps (an update in place through any reference, an assignment, ``load_state_dict(assign=True)``,
+    ``module.to``) is what the step runs with, and no tensor of the caller's is written.  A tensor that is in host memory,
+    or of another type, when the stage is built becomes fp32 on the device first (the tensor object stays, as parameters
+    stay when they move into the arena), so that the copies are between device buffers."""
 
     def __init__(self, blocks: Sequence[nn.Module], device: torch.device):
         self._entries: Dict[Tuple[int, str], Tuple[nn.Module, str, torch.Tensor]] = {}
         for blk in blocks:
             for module, name, shape in getattr(blk, "_pp_live_buffers", lambda: [])():
-                storage = torch.empty(shape, dtype=torch.float32, device=device)
-                self._entries[(id(module), name)] = (module, name, storage)
+                copy = torch.empty(shape, dtype=torch.float32, device=device)
+                self._entries[(id(module), name)] = (module, name, copy)
+                now = self._current(module, name, copy)
+                if now.device.type != copy.device.type or now.dtype != copy.dtype:
+                    now.data = now.detach().to(device=device, dtype=torch.float32)
         self.follow()
-        for module, name, storage in self._entries.values():
-            getattr(module, name).data = storage
 
-    def storage(self, module: nn.Module, name: str) -> torch.Tensor:
+    @staticmethod
+    def _current(module: nn.Module, name: str, copy: torch.Tensor) -> torch.Tensor:
+        now = getattr(module, name, None)
+        if not isinstance(now, torch.Tensor) or now.shape != copy.shape:
+            raise RuntimeError(f"{name} must be a tensor of shape {list(copy.shape)}, not "
+                               f"{list(now.shape) if isinstance(now, torch.Tensor) else now}")
+        return now
+
+    def read_by_lists(self, module: nn.Module, name: str) -> torch.Tensor:
         return self._entries[(id(module), name)][2]
 
     def follow(self) -> None:
-        for module, name, storage in self._entries.values():
-            now = getattr(module, name, None)
-            if not isinstance(now, torch.Tensor) or now.shape != storage.shape:
-                raise RuntimeError(f"{name} must be a tensor of shape {list(storage.shape)}, not "
-                                   f"{list(now.shape) if isinstance(now, torch.Tensor) else now}")
-            if now.data_ptr() != storage.data_ptr() or now.dtype != storage.dtype or now.stride() != storage.stride():
-                storage.copy_(now.detach())
+        for module, name, copy in self._entries.values():
+            copy.copy_(self._current(module, name, copy).detach())
 
 
 class StageProgram:
@@ -1106,7 +1111,7 @@ class StageProgram:
 
     def live_buffer(self, module: nn.Module, name: str) -> torch.Tensor:
         """Where the launch lists read buffer ``name`` of ``module`` (see ``LiveBuffers``)."""
-        return self.live_buffers.storage(module, name)
+        return self.live_buffers.read_by_lists(module, name)
 
     def ones_f32(self, n: int) -> torch.Tensor:
         """A [1, n] row of ones (the left operand that turns an fp32 GEMM into a column sum)."""

@@ -147,6 +147,22 @@ def test_a_tensor_assigned_as_balancing_bias_stays_where_it_is_and_is_read_anew_
         assert all(layer.block_sparse_moe.balance_bias is bias and bias.device.type == "cpu"
                    for layer, bias in zip(model.h, own))
 
+def test_a_balancing_bias_that_was_put_aside_keeps_its_values():
+    model = moe_model()
+    stages, step = moe_pipeline(model)
+    first = [layer.block_sparse_moe.balance_bias for layer in model.h]
+    step()
+    for l, layer in enumerate(model.h):
+        layer.block_sparse_moe.balance_bias = first[l] + pushing(4 + l).to(first[l].device)
+    step()
+    selected_under(stages, [pushing(4), pushing(5)])
+    for layer, bias in zip(model.h, first):
+        assert bool((bias == 0).all())
+        layer.block_sparse_moe.balance_bias = bias
+    step()
+    selected_under(stages, [torch.zeros(E)] * L)
+
+
 # ---- the dropout rate of a layer ------------------------------------------------------------------------------
 def dropout_pipeline(**options):
     import pippy_amd as pp
