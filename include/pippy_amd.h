@@ -519,8 +519,9 @@ int pp_attn_bwd(const pp_attn_desc* desc, pp_stream stream);
  * Attention over packed sequences of different lengths (what a stage module computes per sequence with
  * F.scaled_dot_product_attention, pippy/_PipelineStage.py:420-428, backward pippy/_backward.py:67-69, without the
  * padding that equal lengths would need).  The T rows hold n_seq sequences one after the other, sequence b in rows
- * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (ascending int32 in device memory; empty sequences are fine; bounds out of
- * order or outside [0, T] make an empty sequence).  Any length from 1; causal: query i of a sequence sees its keys
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (ascending int32 in device memory; empty sequences are fine; a pair of bounds
+ * out of order or outside [0, T] makes an empty sequence; what rows hold that two sequences then share, or how many of
+ * them are computed, is not said).  Any length from 1; causal: query i of a sequence sees its keys
  * 0 .. i, else all its keys.  Rows that belong to no sequence are neither read nor written.
  * q: bf16, element (t, h, d) at q + t * stride_q + h * D + d, likewise o, d_o, dq (H heads) and k, v, dk, dv (Hkv
  * heads; query head h reads key / value head h / (H / Hkv), whose gradients are sums over the group in ascending

@@ -1162,8 +1162,8 @@ static int packed_bwd(const pp_attn_packed_desc* d, hipStream_t st) {
         const int rc = packed_launch<attn_packed_bwd_dq_kernel<D, CAUSAL>>("attn_packed_bwd_dq_kernel", 256, blocks64 * d->H,
                                                                            lds + DS * kTile * 2, st, a);
         if (rc) return rc;
-        // Whole backward, us, 64 | 128 keys per work-group: [32 query, 8 key / value heads] T = 2048: 187 | 262, 4096: 483 |
-        // 599, 8192: 1794 | 1721, 16384 in 16 sequences: 649 | 594; [32, 32] T = 1024: 61.5 | 63.7, 2048: 166 | 147
+        // Whole backward, causal, us, 64 | 128 keys per work-group: [32 query, 8 key / value heads] T = 2048: 202 | 272, 4096: 555 |
+        // 668, 8192: 2096 | 2022, in 5 sequences: 625 | 644, 16384 in 16: 963 | 885; [32, 32] T = 1024: 64 | 66, 2048: 176 | 160
         if (packed_wide(d, d->Hkv))
             return packed_launch<attn_packed_bwd_dkv8_kernel<D, CAUSAL, 2>>("attn_packed_bwd_dkv8_kernel", 512,
                                                                             blocks128 * d->Hkv, dkv8_lds_bytes(D, 2), st, a);
