@@ -1072,6 +1072,7 @@ static int packed_check(const char* who, const pp_attn_packed_desc* d, bool bwd)
         {d->v, d->stride_v, d->Hkv * d->D, "v", true},   {d->o, d->stride_o, d->H * d->D, "o", true},
         {d->d_o, d->stride_do, d->H * d->D, "d_o", bwd}, {d->dq, d->stride_dq, d->H * d->D, "dq", bwd},
         {d->dk, d->stride_dk, d->Hkv * d->D, "dk", bwd}, {d->dv, d->stride_dv, d->Hkv * d->D, "dv", bwd}};
+    if (d->T == 0) return PP_OK;  // (empty tensors have no address)
     for (const auto& r : rows) {
         if (!r.need) continue;
         if (!r.p || !aligned(r.p, 16)) return fail(PP_ERR_INVALID, "%s: %s must be a 16-byte aligned pointer", who, r.name);

@@ -928,7 +928,7 @@ static int route_check(const char* who, const pp_moe_route_desc* d) {
     if (d->scoring != PP_MOE_SOFTMAX && d->scoring != PP_MOE_SIGMOID)
         return fail(PP_ERR_INVALID, "%s: unknown scoring %d", who, d->scoring);
     if (d->dtype != PP_BF16 && d->dtype != PP_F32) return fail(PP_ERR_INVALID, "%s: unknown dtype %d", who, d->dtype);
-    if (!d->logits || !d->topk_idx) return fail(PP_ERR_INVALID, "%s: null pointer", who);
+    if (d->T > 0 && (!d->logits || !d->topk_idx)) return fail(PP_ERR_INVALID, "%s: null pointer", who);
     if (!(d->scale == d->scale) || d->scale == INFINITY || d->scale == -INFINITY)
         return fail(PP_ERR_INVALID, "%s: scale must be finite", who);
     return PP_OK;
@@ -946,8 +946,8 @@ extern "C" int pp_moe_route(const pp_moe_route_desc* d, pp_stream stream) {
         (d->group_score != PP_MOE_GROUP_MAX && d->group_score != PP_MOE_GROUP_TOP2))
         return fail(PP_ERR_INVALID, "pp_moe_route: bad groups (%d of %d groups of %d experts for %d slots; at most %d groups)",
                     d->topk_group, d->n_group, d->E, d->topk, kRouteMaxGroups);
+    if (d->T == 0) return PP_OK;  // (empty tensors have no address)
     if (!d->gate) return fail(PP_ERR_INVALID, "pp_moe_route: null pointer");
-    if (d->T == 0) return PP_OK;
     RouteArgs a;
     a.logits = d->logits; a.ld = d->ld; a.T = d->T; a.bias = d->bias;
     a.E = d->E; a.K = d->topk; a.n_group = ng; a.topk_group = kg;
@@ -969,6 +969,7 @@ extern "C" int pp_moe_route(const pp_moe_route_desc* d, pp_stream stream) {
 extern "C" int pp_moe_route_bwd(const pp_moe_route_desc* d, pp_stream stream) {
     const int rc = route_check("pp_moe_route_bwd", d);
     if (rc) return rc;
+    if (d->T == 0) return PP_OK;
     if (!d->dlogits || d->cols_dl < d->E || d->cols_dl > kRouteMaxE || d->ld_dl < d->cols_dl)
         return fail(PP_ERR_INVALID, "pp_moe_route_bwd: bad dlogits (cols=%d ld=%lld for %d experts)", d->cols_dl,
                     (long long)d->ld_dl, d->E);
@@ -978,7 +979,6 @@ extern "C" int pp_moe_route_bwd(const pp_moe_route_desc* d, pp_stream stream) {
             return fail(PP_ERR_INVALID, "pp_moe_route_bwd: needs dgate, or dout, y and pos (16-byte aligned, widths and "
                         "leading dimensions multiples of 8; C=%lld)", (long long)d->C);
     }
-    if (d->T == 0) return PP_OK;
     RouteBwdArgs a;
     a.logits = d->logits; a.ld = d->ld; a.T = d->T; a.E = d->E; a.K = d->topk; a.renorm = d->renorm; a.scale = d->scale;
     a.idx = d->topk_idx; a.dgate = d->dgate;

@@ -223,3 +223,23 @@ def test_permutation_on_either_side_of_its_borders(n, E):
     assert seg.tolist() == [0] + counts.cumsum(0).tolist()
     assert torch.equal(row_src[:len(order)].cpu().long(), order) and bool((row_src[len(order):] == -7).all())
     assert torch.equal(pos.cpu()[order].long(), torch.arange(len(order))) and bool((pos.cpu()[~kept] == -1).all())
+
+
+def test_batches_without_tokens():
+    N = native()
+    q, k = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=DEV), torch.empty(0, 2, 64, dtype=torch.bfloat16, device=DEV)
+    stat = torch.empty(4, 0, device=DEV)
+    for bounds in ([0], [0, 0, 0]):
+        plan = N.attn_packed_plan(torch.tensor(bounds, dtype=torch.int32, device=DEV), 0)
+        N.attn_packed_fwd(q, k, k, torch.empty_like(q), stat, plan)
+        N.attn_packed_bwd(q, k, k, q, stat, q, torch.empty_like(q), torch.empty_like(k), torch.empty_like(k),
+                          torch.empty_like(stat), plan)
+    x, idx, gate = torch.empty(0, 16, device=DEV), torch.empty(0, 2, dtype=torch.int32, device=DEV), torch.empty(0, 2, device=DEV)
+    rows = torch.empty(0, 64, dtype=torch.bfloat16, device=DEV)
+    N.moe_route(x, idx, gate)
+    N.moe_route_bwd(x, idx, torch.empty_like(x), dgate=gate)
+    N.moe_route_bwd(x, idx, torch.empty_like(x), dout=rows, y=rows, pos=idx.view(-1))
+    seg, none = torch.full((17,), 9, dtype=torch.int32, device=DEV), torch.empty(0, dtype=torch.int32, device=DEV)
+    N.moe_permute_ws(idx.view(-1), 16, seg, none, none, torch.empty(N.moe_permute_workspace(0, 16), dtype=torch.int32, device=DEV))
+    assert bool((seg == 0).all())
+    N.dropout_add(rows, torch.empty_like(rows), torch.zeros(2, dtype=torch.int64, device=DEV), 0.1, resid=rows)
