@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd_kernel(c
 // blocks of 64: twice the products per staged block and barrier, half the passes over keys and values, and no merge.
 // Bound by the matrix cores beside the exponentials: causal [8192 rows, 32 query and 8 key / value heads of 128] 519 us =
 // 1060 TFLOP/s of the products it forms (a library product of 8192^3 reaches 1211), 57 % of the cycles in the matrix
-// cores, no LDS conflicts; 16384 rows in 3 sequences, 783 to 870 us.
+// cores, no LDS conflicts; 16384 rows in 3 sequences, 797 to 885 us.
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_fwd128_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -505,7 +505,8 @@ __device__ __forceinline__ float packed_delta(const uint16_t* qp, const uint16_t
 // documents, 12 heads of 64: whole backward 40 -> 42 us; 8192 rows in 5 documents, 32 / 8 heads of 128: 548 -> 638 us, where its
 // registers also end a form of 128 rows per work-group (with it 1118 us with spills, 671 with one wave per SIMD).
 // For head dimension 128 the rows of dO lie in LDS for want of registers (in registers 668 us).
-// In a block with one block of keys D is formed before dS.  Bound like the forward's form of 64 rows.
+// In a block with one block of keys D is formed before dS.  Bound like the forward's form of 64 rows: 20.4 us for the first of
+// these, 305 to 315 for the second (71 % of a library product's rate, 57 % of the cycles in the matrix cores).
 template <int D, bool CAUSAL>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kernel(const PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32, DS = D / 64, NS = attn_stages(D);
@@ -867,7 +868,7 @@ __global__ __launch_bounds__(256, 3) void attn_packed_bwd_dkv_kernel(const Packe
 // other's exponentials; to fit the registers of that the value rows stay in LDS.  KB blocks of 64 keys per
 // work-group: 2, as 4 groups of 32 keys x 2 parts of a step of 64 queries, or 1, as 2 groups x 4 parts of 128
 // queries: twice the work-groups with half the steps each, for launches that would not fill the CUs.  Four
-// products per pair of blocks and the exponentials again; 333 us for causal [8192 rows in 5 documents, 32 query and 8
+// products per pair of blocks and the exponentials again; 333 to 350 us for causal [8192 rows in 5 documents, 32 query and 8
 // key / value heads], 57 % of the cycles in the matrix cores.  Bound by LDS reads beside those; two waves per SIMD is
 // what the registers allow.
 template <int D, bool CAUSAL, int KB>

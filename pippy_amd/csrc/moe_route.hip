@@ -141,7 +141,8 @@ __device__ __forceinline__ double route_sum64(const RouteArgs& a, int64_t t, int
 // 64 experts and K > 4, ranks inside a short list, whose cost hardly grows with K.  us, rounds | list, 8192 tokens,
 // without a bias: E = 64, K = 4: 4.4 | 4.8, 8: 5.6 | 5.6, 16: 7.8 | 14.2 (so 8 lanes have no list); E = 128, K = 4: 4.9 | 5.2,
 // 6: 5.6 | 5.3, 16: 9.5 | 6.6; E = 256, K = 8: 8.2 | 6.3; E = 512, K = 8: 12.6 | 8.0, 16: 19.2 | 9.0.  With a bias E = 256, K = 8:
-// 11.2 | 8.8, in 8 groups, 4 of them kept: 13.2 | 9.4 to 10.9 (8.9 MB: 1.8 us of memory time).
+// 11.2 | 8.8, in 8 groups, 4 of them kept: 13.2 | 9.4 to 11.7 (8.9 MB: 1.8 us of memory
+// time; the same with no choice left to 64 bits as with the usual one in a thousand).
 // Bound by instructions (a round is about 5 V + 30 for 64 / G tokens a wave) and, below a few thousand tokens, by
 // latency (16 experts with K = 2 take 3.4 us).  16 lanes of 16 experts for E = 256 make a round four tokens' worth of
 // work per wave; a wave per token spends most of a round on the reductions.
