@@ -527,7 +527,7 @@ int pp_attn_bwd(const pp_attn_desc* desc, pp_stream stream);
  * heads; query head h reads key / value head h / (H / Hkv), whose gradients are sums over the group in ascending
  * head order).  Row strides are multiples of 8 elements, at most 2^23, pointers 16-byte aligned: q, k, v may be
  * sections of one projection's rows.  lse, delta: fp32 [H, T] (log-sum-exp of the scaled scores, saved for the
- * backward; the backward's row sums of P dP).  D 64 or 128.  scale between 2^-64 and 2^64.  Softmax statistics and
+ * backward; the backward's row sums of P dP over those of P).  D 64 or 128.  scale between 2^-64 and 2^64.  Softmax statistics and
  * all sums are fp32; P and dS are rounded to bf16 as operands of their products.  The rounding of the stored output does
  * not reach the gradients: they are formed with the row sums of P dP (for dq as PP_ATTN_EXACT_DQ does).  No atomics:
  * the same bits on every run.

@@ -495,7 +495,9 @@ __device__ __forceinline__ float packed_delta(const uint16_t* qp, const uint16_t
 }
 
 // A work-group owns 64 query rows (2 groups of 32 queries x 2 halves of every key block) and hands the dK / dV
-// kernel the row sums D = sum_j P dP.
+// kernel the row sums D = sum_j P dP.  P comes from the stored log-sum-exp, whose rounding, 2^-24 of a number that may be some
+// thousands, is one factor on all weights of a row.  From 16 on (a factor of 1 + 2^-20), and with few keys, D is divided by
+// sum_j P, so that the row of dS sums to zero all the same.  (Only there: the sum costs up to 2.5 % of the backward.)
 //
 // dS = P (dP - D), but D is known only behind the loop.  The loop takes delta = rowsum(dO O) of the stored output for it, which
 // the rounding of the output keeps from D by r = D - delta, and so leaves a surplus of r P k_j for every key: r times the
@@ -544,7 +546,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         lo.load(Ol, q0, wave);
     }
     const float lse_q = a.lse[(int64_t)w.h * a.T + row] * kLog2e;
-    float d_sum = 0.f;  // D
+    float d_sum = 0.f, p_sum = 0.f;
+    const bool divide = n_blocks == 1 || __any(fabsf(lse_q) > 16.f * kLog2e);  // (the waves of a group have the same queries)
 #pragma unroll
     for (int t = 0; t < NS - 1; ++t)
         if (t < n_blocks) issue(t, t);
@@ -589,6 +592,21 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         }
 #pragma unroll
         for (int v = 0; v < 16; ++v) d_sum = fmaf(dsv[v], dpacc[v], d_sum);
+        if (divide) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) p_sum += dsv[v];
+        }
+    };
+    // the row's D from the sums of its lanes and waves; `part`: 256 floats that no load and no other wave uses
+    auto row_sum = [&](float* part) __attribute__((always_inline)) {
+        d_sum += __shfl_xor(d_sum, 32, 64);
+        p_sum += __shfl_xor(p_sum, 32, 64);
+        part[wave * 64 + lane] = lh == 0 ? d_sum : p_sum;
+        wait_lds();
+        __syncthreads();
+        const float* row = part + grp * 64 + l32;
+        const float d = row[0] + row[128];
+        return divide ? d / (row[32] + row[160]) : d;
     };
     auto step = [&](auto masked_c, const uint16_t* Ks, int j) __attribute__((always_inline)) {
         float dsv[16];
@@ -625,13 +643,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         float pv[16];
         f32x16_t dpv;
         if (sees) weights(std::true_type{}, Ks, 0, pv, dpv);
-        d_sum += __shfl_xor(d_sum, 32, 64);
-        float* part = reinterpret_cast<float*>(lds + kStage);  // the second stage, which nothing was loaded into
-        if (lh == 0) part[wave * 32 + l32] = d_sum;
-        wait_lds();
-        __syncthreads();
-        delta_q = part[grp * 32 + l32] + part[(2 + grp) * 32 + l32];
-        d_sum = 0.f;
+        delta_q = row_sum(reinterpret_cast<float*>(lds + kStage));  // the second stage, which nothing was loaded into
+        d_sum = p_sum = 0.f;
         if (sees) step(std::true_type{}, Ks, 0);
         j = 1;
     }
@@ -641,16 +654,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
         const int kt0 = j * 64 + 32 * half;
         if (kt0 < w.len && (!CAUSAL || kt0 <= qw0 + 31)) step(std::true_type{}, Ks, j);
     }
-    d_sum += __shfl_xor(d_sum, 32, 64);
     // add the sums of the two halves, first the row sums, then [grp][16 DT values][64 lanes] floats
-    float* rows = reinterpret_cast<float*>(lds) + 2 * 16 * DT * 64;
     float* xs = reinterpret_cast<float*>(lds) + grp * (16 * DT * 64) + lane;
     wait_lds();
     __syncthreads();
-    rows[wave * 64 + lane] = d_sum;
-    __syncthreads();
-    d_sum += rows[(wave ^ 2) * 64 + lane];
-    const float r = d_sum - delta_q;
+    const float d_row = row_sum(reinterpret_cast<float*>(lds) + 2 * 16 * DT * 64);
+    const float r = d_row - delta_q;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -663,7 +672,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_packed_bwd_dq_kerne
     }
     __syncthreads();
     if (half == 1 || qi >= w.len) return;
-    if (lh == 0) a.delta[(int64_t)w.h * a.T + row] = d_sum;
+    if (lh == 0) a.delta[(int64_t)w.h * a.T + row] = d_row;
     uint16_t* dqp = a.dq + row * a.sdq + (int64_t)w.h * D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)

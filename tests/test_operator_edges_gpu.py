@@ -243,3 +243,43 @@ def test_batches_without_tokens():
     N.moe_permute_ws(idx.view(-1), 16, seg, none, none, torch.empty(N.moe_permute_workspace(0, 16), dtype=torch.int32, device=DEV))
     assert bool((seg == 0).all())
     N.dropout_add(rows, torch.empty_like(rows), torch.zeros(2, dtype=torch.int64, device=DEV), 0.1, resid=rows)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens", [[1, 1, 2, 3, 1], [40, 2, 130], [1, 300]])
+@pytest.mark.parametrize("causal", [False, True])
+def test_query_and_key_gradients_under_large_scores(D, lens, causal):
+    """Scores of some thousands: fp32 holds a row's log-sum-exp to 2^-24 of that, so all its weights are off by one factor,
+    which must not show: the row sum is of weights that sum to one.  What may show: fp32 errors of the single scores, e =
+    (D + 8) 2^-24 of sum |q| |k|, which shift weights against each other and enter dS as P 2 e (|dP - D| + sum P |dP - D|); those
+    of the products dP, (D + 8) 2^-24 of sum |dO| |V|, and of the row sum, 2^-20 of sum P |dP|; dS and the results in bf16."""
+    N = native()
+    H, T = 4, sum(lens)
+    g = torch.Generator().manual_seed(T + D)
+    common = torch.randn(2, 1, H, D, generator=g) * 4
+    q = (torch.randn(T, H, D, generator=g) * 16).to(torch.bfloat16)
+    k, v = (torch.randn(2, T, H, D, generator=g) + common).to(torch.bfloat16).unbind(0)
+    q[:, 0] = (8 * common[0, :, 0]).to(torch.bfloat16)              # one head with scores far from zero on one side
+    do = torch.randn(T, H, D, generator=g).to(torch.bfloat16)
+    qd, kd, vd, dod = (t.to(DEV) for t in (q, k, v, do))
+    o, dq, dk, dv = (torch.empty_like(qd) for _ in range(4))
+    lse, delta = (torch.empty(H, T, device=DEV) for _ in range(2))
+    cu = [0] + torch.tensor(lens).cumsum(0).tolist()
+    plan = N.attn_packed_plan(torch.tensor(cu, dtype=torch.int32, device=DEV), T)
+    N.attn_packed_fwd(qd, kd, vd, o, lse, plan, causal=causal)
+    N.attn_packed_bwd(qd, kd, vd, o, lse, dod, dq, dk, dv, delta, plan, causal=causal)
+    scale = D ** -0.5
+    for a, b in zip(cu[:-1], cu[1:]):
+        Q, K, V, dO = (t[a:b].double().transpose(0, 1) for t in (q, k, v, do))
+        hidden = torch.ones(b - a, b - a, dtype=torch.bool).triu(1) if causal else torch.zeros(b - a, b - a, dtype=torch.bool)
+        P = torch.softmax((Q @ K.transpose(1, 2) * scale).masked_fill(hidden, float("-inf")), -1)
+        dP = dO @ V.transpose(1, 2)
+        off = dP - (P * dP).sum(-1, keepdim=True)
+        dS = P * off
+        e = ((D + 8) * 2.0 ** -24 * (Q.abs() @ K.abs().transpose(1, 2)) * scale).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+        dp_err = (D + 8) * 2.0 ** -24 * (dO.abs() @ V.abs().transpose(1, 2))
+        err = U * dS.abs() + P * (2 * e * (off.abs() + dS.abs().sum(-1, keepdim=True)) + dp_err
+                                  + (P * dp_err).sum(-1, keepdim=True) + 2.0 ** -20 * (P * dP.abs()).sum(-1, keepdim=True))
+        for name, got, want, bound in (("dq", dq, dS @ K * scale, scale * err @ K.abs()),
+                                       ("dk", dk, dS.transpose(1, 2) @ Q * scale, scale * err.transpose(1, 2) @ Q.abs())):
+            within(got[a:b].transpose(0, 1), want, 1.02 * (bound + U * want.abs()) + 1e-30, f"{name} of rows {a} to {b - 1}")
